@@ -188,7 +188,7 @@ def _quantised(y: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """y [pages, heads, page, d] as MXFP4: codes [pages, heads, page, d / 2] and scales [pages, heads, d / 32, page]."""
     blocks = y.unflatten(-1, (-1, 32))
     top = blocks.abs().amax(-1)
-    exponent = (torch.frexp(top).exponent - 3).clamp(min=-126)
+    exponent = torch.where(top > 0, torch.frexp(top).exponent - 3, -126).clamp(min=-126)
     fine = top.isfinite()
     scale = torch.where(fine, exponent + 127, 255).to(torch.uint8)
     m = torch.ldexp(blocks.abs(), -exponent[..., None])
