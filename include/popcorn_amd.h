@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define PK_ABI_VERSION 5
+#define PK_ABI_VERSION 6
 
 /* status codes */
 #define PK_OK 0
@@ -317,6 +317,98 @@ int pk_attn_varlen_bwd(const void* q, const void* k, const void* v, const void* 
                        void* workspace, int64_t workspace_bytes, void* dq, void* dk, void* dv, const int* cu_seqlens,
                        const int64_t* strides, int64_t num_seqs, int64_t total, int64_t max_seqlen, int64_t q_heads,
                        int64_t kv_heads, int64_t head_dim, float softmax_scale, int causal, int dtype, void* stream);
+
+/*
+ * Paged caches of keys and values, for the four entry points below. A cache is
+ * a pool of num_pages pages of page_size tokens (a multiple of 16):
+ *   rows of q's type   [num_pages, kv_heads, page_size, head_dim]
+ *   MXFP4 codes        [num_pages, kv_heads, page_size, head_dim / 2] bytes, two
+ *                      e2m1 codes each, the even channel in the low nibble
+ *   MXFP4 scales       [num_pages, kv_heads, head_dim / 32, page_size] bytes, the
+ *                      E8M0 exponent of each 32 channels (2^(byte - 127); 255 is
+ *                      NaN), a page's tokens contiguous
+ * with any strides for the other dimensions, the last one contiguous. They have
+ * no counterpart in the reference, whose attention covers whole sequences
+ * (kernels/attn.py:10-37); they stand beside `rope` (kernels/rope.py:19-36) and
+ * `attn_varlen` (kernels/attn_varlen.py:15-54).
+ */
+
+/*
+ * Rotates the queries and keys of `tokens` new tokens and appends their keys and
+ * values to the cache, in one launch: token t at positions[t] (rows of cos, sin
+ * [max_positions, half], contiguous; clamped to them) goes to row slots[t] % page_size
+ * of page slots[t] / page_size. A slot below 0 or past the pool is not written, and
+ * no two tokens may have the same one. q [tokens, q_heads, head_dim], k and v
+ * [tokens, kv_heads, head_dim]; yq and yk contiguous receive the rotated q and k.
+ * Pairs, channels past 2*half and arithmetic as pk_rotary. positions and slots are
+ * int32, or int64 where wide_positions / wide_slots are 1. strides[12] = q, k, v
+ * (token, head), k_cache, v_cache (page, head, token), in elements. head_dim a
+ * multiple of 8 up to 256. Outputs overlap no input.
+ */
+int pk_rope_append(const void* q, const void* k, const void* v, const void* cos, const void* sin, const void* positions,
+                   const void* slots, void* yq, void* yk, void* k_cache, void* v_cache, const int64_t* strides,
+                   int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t half,
+                   int64_t max_positions, int64_t num_pages, int64_t page_size, int dtype, int cs_dtype,
+                   int wide_positions, int wide_slots, int interleaved, void* stream);
+
+/*
+ * The same into an MXFP4 cache. A block of 32 channels with the largest magnitude a
+ * has the scale 2^max(floor(log2 a) - 2, -126), and its values are the nearest of
+ * 0, .5, 1, 1.5, 2, 3, 4, 6 scales (ties to even, over 6 to 6). Rotated keys are
+ * quantised as their exact 64-bit sums, without a rounding before it. A block that
+ * holds a NaN, an Inf or a magnitude past fp32 is NaN. yk and yv (contiguous, q's type) receive what the
+ * cache's rows now stand for (also of tokens that are not written), rounded to q's
+ * type. head_dim a multiple of 32 up to 256. strides[18] = q, k, v (token, head),
+ * k_codes, v_codes (page, head, token), k_scales, v_scales (page, head, block).
+ */
+int pk_rope_append_mxfp4(const void* q, const void* k, const void* v, const void* cos, const void* sin,
+                         const void* positions, const void* slots, void* yq, void* yk, void* yv, void* k_codes,
+                         void* k_scales, void* v_codes, void* v_scales, const int64_t* strides, int64_t tokens,
+                         int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t half, int64_t max_positions,
+                         int64_t num_pages, int64_t page_size, int dtype, int cs_dtype, int wide_positions,
+                         int wide_slots, int interleaved, void* stream);
+
+/*
+ * Bytes of device workspace pk_attn_paged (mxfp4 = 0) or pk_attn_paged_mxfp4 (1)
+ * needs for this shape on the current device (`packed`: with cu_seqlens; capacity =
+ * table_width * page_size), 0 where no sequence can be split, -1 for an invalid shape.
+ */
+int64_t pk_attn_paged_workspace(int64_t num_seqs, int64_t total, int packed, int64_t q_heads, int64_t kv_heads,
+                                int64_t head_dim, int64_t capacity, int dtype, int mxfp4);
+
+/*
+ * Attention of new tokens over a paged cache, grouped-query. Sequence i has the
+ * tokens [cu_seqlens[i], cu_seqlens[i+1]) of q [total, q_heads, head_dim] (n of them;
+ * cu_seqlens NULL: token i alone, total = num_seqs) and the first L = cache_lens[i]
+ * keys of pages block_table[i][0], block_table[i][1], ..., the new tokens' own
+ * included. Token t of n attends keys 0 .. L - n + t (causal), or all L. o is
+ * contiguous like q; a token that attends no key gets zeros, and so does one that no
+ * sequence holds. Keys on a table entry outside [0, num_pages) are left out, and
+ * lengths past the table's capacity are cut to it. block_table [num_seqs, table_width]
+ * (rows table_stride apart), cache_lens and cu_seqlens are int32 device arrays;
+ * nothing is read back, so a captured call may be replayed with other contents.
+ * What the pages hold behind a sequence's keys is not looked at. strides[8] = q
+ * (token, head), k_cache, v_cache (page, head, token), in elements, multiples of
+ * 16 bytes like every pointer. head_dim a multiple of 8 up to 256. workspace:
+ * pk_attn_paged_workspace() bytes, 16-byte aligned.
+ */
+int pk_attn_paged(const void* q, const void* k_cache, const void* v_cache, const int* block_table, const int* cache_lens,
+                  const int* cu_seqlens, void* o, void* workspace, int64_t workspace_bytes, const int64_t* strides,
+                  int64_t num_seqs, int64_t total, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                  int64_t num_pages, int64_t page_size, int64_t table_width, int64_t table_stride, float softmax_scale,
+                  int causal, int dtype, void* stream);
+
+/*
+ * The same over an MXFP4 cache, for q of any dtype: strides[14] = q (token, head),
+ * k_codes, v_codes (page, head, token, multiples of 16 bytes), k_scales, v_scales
+ * (page, head, block, multiples of 4). head_dim a multiple of 32 up to 256.
+ */
+int pk_attn_paged_mxfp4(const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
+                        const void* v_scales, const int* block_table, const int* cache_lens, const int* cu_seqlens,
+                        void* o, void* workspace, int64_t workspace_bytes, const int64_t* strides, int64_t num_seqs,
+                        int64_t total, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t num_pages,
+                        int64_t page_size, int64_t table_width, int64_t table_stride, float softmax_scale, int causal,
+                        int dtype, void* stream);
 
 /*
  * Matrix-core rate probe, a measurement aid with no counterpart in the

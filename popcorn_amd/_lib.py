@@ -16,7 +16,7 @@ from pathlib import Path
 import torch
 
 LIBRARY = Path(__file__).resolve().parent / "libpopcorn_amd.so"
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_HIP = 0, 1, 2, 3
 F32, BF16, F16 = 0, 1, 2
@@ -53,6 +53,11 @@ SIGNATURES = {
     "pk_attn_varlen_bwd_workspace": (_i64, [_i64] * 6),
     "pk_attn_varlen_bwd": (_int, [_p] * 7 + [_i64] + [_p] * 5 + [_i64] * 6 + [_f32, _int, _int, _p]),
     "pk_attn_varlen_fwd": (_int, [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _int, _int, _p]),
+    "pk_rope_append": (_int, [_p] * 11 + [_p] + [_i64] * 8 + [_int] * 5 + [_p]),
+    "pk_rope_append_mxfp4": (_int, [_p] * 14 + [_p] + [_i64] * 8 + [_int] * 5 + [_p]),
+    "pk_attn_paged_workspace": (_i64, [_i64, _i64, _int, _i64, _i64, _i64, _i64, _int, _int]),
+    "pk_attn_paged": (_int, [_p] * 8 + [_i64, _p] + [_i64] * 9 + [_f32, _int, _int, _p]),
+    "pk_attn_paged_mxfp4": (_int, [_p] * 10 + [_i64, _p] + [_i64] * 9 + [_f32, _int, _int, _p]),
     "pk_probe_mfma": (_int, [_int, _int, _int, _p, _p]),
     "pk_probe_stream": (_int, [_p, _p, _p, _i64, _int, _p]),
 }

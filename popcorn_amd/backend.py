@@ -168,7 +168,123 @@ def attn_varlen_supported(q, k, v, cu_seqlens, causal, softmax_scale) -> bool:
     )
 
 
-# (op, source, predicate, forward_only): every op has its backward kernels.
+def _cache_supported(head_dim: int, kv_heads: int, *rows) -> bool:
+    """Caches [pages, kv_heads, page_size, row] of one shape, rows contiguous, page_size a multiple of 16."""
+    return (
+        all(t.dim() == 4 and t.shape == rows[0].shape and t.stride(-1) == 1 for t in rows)
+        and rows[0].shape[1] == kv_heads
+        and rows[0].shape[2] >= 16
+        and rows[0].shape[2] % 16 == 0
+        and 8 <= head_dim <= 256
+    )
+
+
+def _mxfp4_supported(head_dim: int, kv_heads: int, codes, scales) -> bool:
+    return (
+        all(t.dtype == torch.uint8 for t in codes + scales)
+        and head_dim % 32 == 0
+        and _cache_supported(head_dim, kv_heads, *codes)
+        and 2 * codes[0].shape[3] == head_dim
+        and all(t.dim() == 4 and t.stride(-1) == 1 for t in scales)
+        and all(tuple(t.shape) == (codes[0].shape[0], kv_heads, head_dim // 32, codes[0].shape[2]) for t in scales)
+    )
+
+
+def _append_supported(q, k, v, cos, sin, positions, slots) -> bool:
+    integers = (torch.int32, torch.int64)
+    return (
+        q.dtype in _FLOATS
+        and q.dtype == k.dtype == v.dtype
+        and cos.dtype in _FLOATS
+        and cos.dtype == sin.dtype
+        and q.dim() == k.dim() == 3
+        and k.shape == v.shape
+        and q.shape[0] == k.shape[0]
+        and q.shape[2] == k.shape[2]
+        and cos.dim() == 2
+        and cos.shape == sin.shape
+        and cos.shape[0] > 0
+        and 1 <= cos.shape[1] <= q.shape[2] // 2
+        and positions.dtype in integers
+        and slots.dtype in integers
+        and positions.shape == slots.shape == q.shape[:1]
+    )
+
+
+def _own_memory(*caches) -> bool:
+    return all(stride or size < 2 for t in caches for size, stride in zip(t.shape, t.stride()))
+
+
+def rope_append_supported(q, k, v, cos, sin, positions, slots, k_cache, v_cache, interleaved) -> bool:
+    return (
+        _on_hip(q, k, v, cos, sin, positions, slots, k_cache, v_cache)
+        and _append_supported(q, k, v, cos, sin, positions, slots)
+        and q.dtype == k_cache.dtype == v_cache.dtype
+        and q.shape[2] % 8 == 0
+        and _cache_supported(q.shape[2], k.shape[1], k_cache, v_cache)
+        and k_cache.shape[3] == q.shape[2]
+        and _own_memory(k_cache, v_cache)
+    )
+
+
+def rope_append_mxfp4_supported(q, k, v, cos, sin, positions, slots, k_codes, k_scales, v_codes, v_scales,
+                                interleaved) -> bool:
+    return (
+        _on_hip(q, k, v, cos, sin, positions, slots, k_codes, k_scales, v_codes, v_scales)
+        and _append_supported(q, k, v, cos, sin, positions, slots)
+        and _mxfp4_supported(q.shape[2], k.shape[1], (k_codes, v_codes), (k_scales, v_scales))
+        and _own_memory(k_codes, k_scales, v_codes, v_scales)
+        and _aligned(4, k_codes, v_codes)
+    )
+
+
+def _table_supported(q, cache, block_table, cache_lens, cu_seqlens) -> bool:
+    given = [t for t in (block_table, cache_lens, cu_seqlens) if t is not None]
+    seqs = q.shape[0] if cu_seqlens is None else cu_seqlens.numel() - 1
+    return (
+        q.dtype in _FLOATS
+        and q.dim() == 3
+        and cache.dim() == 4
+        and cache.shape[1] > 0
+        and q.shape[1] % cache.shape[1] == 0
+        and all(t.dtype == torch.int32 for t in given)
+        and block_table.dim() == 2
+        and block_table.shape[0] == seqs
+        and tuple(cache_lens.shape) == (seqs,)
+        and (cu_seqlens is None or cu_seqlens.dim() == 1)
+    )
+
+
+def _aligned(unit: int, *tensors) -> bool:
+    """Every row starts at a multiple of `unit` bytes."""
+    return all(t.data_ptr() % unit == 0 and all(n < 2 or s * t.element_size() % unit == 0
+                                                for n, s in zip(t.shape[:-1], t.stride())) for t in tensors)
+
+
+def attn_paged_supported(q, k_cache, v_cache, block_table, cache_lens, cu_seqlens, causal, softmax_scale) -> bool:
+    return (
+        _on_hip(q, k_cache, v_cache, block_table, cache_lens, cu_seqlens)
+        and _table_supported(q, k_cache, block_table, cache_lens, cu_seqlens)
+        and q.dtype == k_cache.dtype == v_cache.dtype
+        and _attn_head_dim(q.shape[2])
+        and _cache_supported(q.shape[2], k_cache.shape[1], k_cache, v_cache)
+        and k_cache.shape[3] == q.shape[2]
+        and _aligned(16, k_cache, v_cache)
+    )
+
+
+def attn_paged_mxfp4_supported(q, k_codes, k_scales, v_codes, v_scales, block_table, cache_lens, cu_seqlens, causal,
+                               softmax_scale) -> bool:
+    return (
+        _on_hip(q, k_codes, k_scales, v_codes, v_scales, block_table, cache_lens, cu_seqlens)
+        and _table_supported(q, k_codes, block_table, cache_lens, cu_seqlens)
+        and _mxfp4_supported(q.shape[2], k_codes.shape[1], (k_codes, v_codes), (k_scales, v_scales))
+        and _aligned(16, k_codes, v_codes)
+        and _aligned(4, k_scales, v_scales)
+    )
+
+
+# (op, source, predicate, forward_only): every op but the paged cache's has its backward kernels.
 REGISTRATIONS = (
     ("rms_norm", "popcorn_amd.impls.rms_norm", rms_norm_supported, False),
     ("add_rms_norm", "popcorn_amd.impls.add_rms_norm", add_rms_norm_supported, False),
@@ -178,6 +294,10 @@ REGISTRATIONS = (
     ("qk_norm_rope", "popcorn_amd.impls.qk_norm_rope", qk_norm_rope_supported, False),
     ("attn", "popcorn_amd.impls.attn", attn_supported, False),
     ("attn_varlen", "popcorn_amd.impls.attn_varlen", attn_varlen_supported, False),
+    ("rope_append", "popcorn_amd.impls.rope_append", rope_append_supported, True),
+    ("rope_append_mxfp4", "popcorn_amd.impls.rope_append_mxfp4", rope_append_mxfp4_supported, True),
+    ("attn_paged", "popcorn_amd.impls.attn_paged", attn_paged_supported, True),
+    ("attn_paged_mxfp4", "popcorn_amd.impls.attn_paged_mxfp4", attn_paged_mxfp4_supported, True),
 )
 
 
@@ -199,7 +319,7 @@ def register(popcorn: ModuleType | None = None) -> ModuleType:
     pc.declare_backend(BACKEND, package=DISTRIBUTION, min_version=__version__, max_version=__version__)
     for op_name, source, predicate, forward_only in REGISTRATIONS:
         op = pc.KERNELS.get(op_name)
-        if op is None:  # qk_norm_rope exists once defined (Popcorn's notebook does; compat ships it)
+        if op is None:  # qk_norm_rope and the paged cache's ops exist once defined (compat ships them)
             continue
         if BACKEND not in op.available_backends():  # registering twice is a no-op, not an error
             op.register(BACKEND, source=source, predicate=predicate, forward_only=forward_only)

@@ -16,13 +16,13 @@ from popcorn_amd.compat.harness import compare, compare_inputs, report
 from popcorn_amd.compat.ops import KERNELS, Dispatcher, Implementation, register_kernel
 from popcorn_amd.compat.records import Case, Record
 from popcorn_amd.compat.selection import Policy, Range
-from popcorn_amd.compat.shapes import BFloat16, Float, Float16, Float32, Float64, Int32
+from popcorn_amd.compat.shapes import BFloat16, Float, Float16, Float32, Float64, Int, Int32, UInt8
 from popcorn_amd.compat import harness, references, store  # noqa: E402
 from popcorn_amd.compat import kernels  # noqa: E402  registers the transformer-block ops
 
 __all__ = [
     "KERNELS", "Dispatcher", "Implementation", "register_kernel", "BackendUnavailableError", "BackendVersionError",
     "DispatchError", "PopcornError", "compare", "compare_inputs", "report", "Case", "Record", "Policy", "Range",
-    "BFloat16", "Float", "Float16", "Float32", "Float64", "Int32", "declare_backend", "kernel", "kernels", "harness",
+    "BFloat16", "Float", "Float16", "Float32", "Float64", "Int", "Int32", "UInt8", "declare_backend", "kernel", "kernels", "harness",
     "references", "store",
 ]

@@ -12,7 +12,7 @@ from torch import Tensor
 
 from popcorn_amd.compat import references
 from popcorn_amd.compat.ops import register_kernel
-from popcorn_amd.compat.shapes import Float, Int32
+from popcorn_amd.compat.shapes import Float, Int, Int32, UInt8
 
 
 @register_kernel(test_args={"eps": [1e-6, 1e-5]})
@@ -111,3 +111,81 @@ def attn_varlen(
 ) -> Float[Tensor, "total q_heads head_dim"]:
     """Attention over packed variable-length sequences, each attended independently."""
     return references.attn_varlen(q, k, v, cu_seqlens, causal, softmax_scale)
+
+
+# The paged cache's ops: not Popcorn's, in its manner. They write the cache in place and are forward-only.
+
+@register_kernel(test_inputs={"slots": references.distinct_slots}, tags={"positional", "cache"})
+def rope_append(
+    q: Float[Tensor, "tokens q_heads head_dim"],
+    k: Float[Tensor, "tokens kv_heads head_dim"],
+    v: Float[Tensor, "tokens kv_heads head_dim"],
+    cos: Float[Tensor, "max_positions half"],
+    sin: Float[Tensor, "max_positions half"],
+    positions: Int[Tensor, "tokens"],
+    slots: Int[Tensor, "tokens"],
+    k_cache: Float[Tensor, "pages kv_heads page_size head_dim"],
+    v_cache: Float[Tensor, "pages kv_heads page_size head_dim"],
+    interleaved: bool = False,
+) -> tuple[Tensor, Tensor]:
+    """Rotate new queries and keys and append the keys and values to a paged cache: (yq, yk)."""
+    return references.rope_append(q, k, v, cos, sin, positions, slots, k_cache, v_cache, interleaved)
+
+
+@register_kernel(test_inputs={"slots": references.distinct_slots}, tags={"positional", "cache"})
+def rope_append_mxfp4(
+    q: Float[Tensor, "tokens q_heads head_dim"],
+    k: Float[Tensor, "tokens kv_heads head_dim"],
+    v: Float[Tensor, "tokens kv_heads head_dim"],
+    cos: Float[Tensor, "max_positions half"],
+    sin: Float[Tensor, "max_positions half"],
+    positions: Int[Tensor, "tokens"],
+    slots: Int[Tensor, "tokens"],
+    k_codes: UInt8[Tensor, "pages kv_heads page_size packed"],
+    k_scales: UInt8[Tensor, "pages kv_heads blocks page_size"],
+    v_codes: UInt8[Tensor, "pages kv_heads page_size packed"],
+    v_scales: UInt8[Tensor, "pages kv_heads blocks page_size"],
+    interleaved: bool = False,
+) -> tuple[Tensor, Tensor, Tensor]:
+    """`rope_append` into an MXFP4 cache: (yq, yk, yv), the last two what the cache now stands for."""
+    return references.rope_append_mxfp4(q, k, v, cos, sin, positions, slots, k_codes, k_scales, v_codes, v_scales,
+                                        interleaved)
+
+
+@register_kernel(test_args={"softmax_scale": [None, 0.25]},
+                 test_inputs={"block_table": references.table_entries, "cache_lens": references.cached_lengths,
+                              "cu_seqlens": references.cuts},
+                 tags={"cache"})
+def attn_paged(
+    q: Float[Tensor, "total q_heads head_dim"],
+    k_cache: Float[Tensor, "pages kv_heads page_size head_dim"],
+    v_cache: Float[Tensor, "pages kv_heads page_size head_dim"],
+    block_table: Int32[Tensor, "sequences table_pages"],
+    cache_lens: Int32[Tensor, "sequences"],
+    cu_seqlens: Int32[Tensor, "boundaries"] | None = None,
+    causal: bool = True,
+    softmax_scale: float | None = None,
+) -> Float[Tensor, "total q_heads head_dim"]:
+    """Attention of each sequence's new tokens over its pages of a cache of keys and values."""
+    return references.attn_paged(q, k_cache, v_cache, block_table, cache_lens, cu_seqlens, causal, softmax_scale)
+
+
+@register_kernel(test_args={"softmax_scale": [None, 0.25]},
+                 test_inputs={"block_table": references.table_entries, "cache_lens": references.cached_lengths,
+                              "cu_seqlens": references.cuts},
+                 tags={"cache"})
+def attn_paged_mxfp4(
+    q: Float[Tensor, "total q_heads head_dim"],
+    k_codes: UInt8[Tensor, "pages kv_heads page_size packed"],
+    k_scales: UInt8[Tensor, "pages kv_heads blocks page_size"],
+    v_codes: UInt8[Tensor, "pages kv_heads page_size packed"],
+    v_scales: UInt8[Tensor, "pages kv_heads blocks page_size"],
+    block_table: Int32[Tensor, "sequences table_pages"],
+    cache_lens: Int32[Tensor, "sequences"],
+    cu_seqlens: Int32[Tensor, "boundaries"] | None = None,
+    causal: bool = True,
+    softmax_scale: float | None = None,
+) -> Float[Tensor, "total q_heads head_dim"]:
+    """`attn_paged` over an MXFP4 cache."""
+    return references.attn_paged_mxfp4(q, k_codes, k_scales, v_codes, v_scales, block_table, cache_lens, cu_seqlens,
+                                       causal, softmax_scale)

@@ -14,6 +14,9 @@ the native-dtype rounding the budget measures:
     qk_norm_rope      examples/03_write_a_kernel.ipynb, cell 3 (`rms`: kernels/_utils.py:14-16)
     attn              kernels/attn.py:10-37
     attn_varlen       kernels/attn_varlen.py:15-54 (`cuts`: kernels/_varlen.py:8-13)
+
+The paged cache's ops (`rope_append`, `attn_paged` and their MXFP4 forms) are not
+Popcorn's; their references are here in the same manner.
 """
 
 from __future__ import annotations
@@ -178,3 +181,158 @@ def cuts(t: Tensor, dims, generator: torch.Generator) -> Tensor:
         raise ValueError(f"total={total} cannot hold {segments} non-empty segments")
     inner = (torch.randperm(total - 1, generator=generator)[: segments - 1] + 1).sort().values
     return torch.cat([torch.zeros(1, dtype=inner.dtype), inner, torch.full((1,), total, dtype=inner.dtype)]).int()
+
+
+# --------------------------------------------------------------------------- paged cache
+
+
+def _cache_rows(slots: Tensor, pages: int, page_size: int) -> tuple[Tensor, Tensor, Tensor]:
+    """(tokens that are written, their pages, their rows)."""
+    kept = torch.nonzero((slots >= 0) & (slots < pages * page_size))[:, 0]
+    at = slots[kept].long()
+    return kept, torch.div(at, page_size, rounding_mode="floor"), at % page_size
+
+
+def _at_positions(x: Tensor, cos: Tensor, sin: Tensor, positions: Tensor, interleaved: bool) -> Tensor:
+    at = positions.long().clamp(0, cos.shape[0] - 1)
+    return rotary_embedding(x[None], cos[at], sin[at], interleaved)[0]
+
+
+@torch.no_grad()
+def rope_append(q: Tensor, k: Tensor, v: Tensor, cos: Tensor, sin: Tensor, positions: Tensor, slots: Tensor,
+                k_cache: Tensor, v_cache: Tensor, interleaved: bool = False) -> tuple[Tensor, Tensor]:
+    """`rotary_embedding` of every token at its position; keys and values written to their cache rows, in place."""
+    yq, yk = (_at_positions(t, cos, sin, positions, interleaved) for t in (q, k))
+    kept, page, row = _cache_rows(slots, k_cache.shape[0], k_cache.shape[2])
+    k_cache[page, :, row] = yk[kept]
+    v_cache[page, :, row] = v[kept]
+    return yq, yk
+
+
+E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def mxfp4_encode(y: Tensor) -> tuple[Tensor, Tensor]:
+    """y [..., d] (rounded no further than float64) as codes [..., d / 2] and scale bytes [..., d / 32], both uint8.
+
+    A block of 32 takes the scale 2^max(floor(log2 max|y|) - 2, -126); its values go to the
+    nearest of E2M1, ties to the even code. A block with a value fp32 does not hold is NaN (255).
+    """
+    blocks = y.double().unflatten(-1, (-1, 32))
+    top = blocks.abs().amax(-1, keepdim=True)
+    fine = top <= torch.finfo(torch.float32).max
+    exponent = torch.where(top > 0, torch.frexp(top).exponent - 3, -126).clamp(min=-126)
+    m = torch.ldexp(torch.where(fine, blocks.abs(), 0.0), -exponent)
+    borders = [(a + b) / 2 for a, b in zip(E2M1, E2M1[1:])]
+    code = sum((m >= b) if i % 2 else (m > b) for i, b in enumerate(borders)) + 8 * blocks.signbit().long()
+    code = torch.where(fine, code, 0).to(torch.uint8).flatten(-2)
+    scale = torch.where(fine, exponent + 127, 255).to(torch.uint8)[..., 0]
+    return code[..., 0::2] | code[..., 1::2] << 4, scale
+
+
+def mxfp4_decode(codes: Tensor, scales: Tensor) -> Tensor:
+    """float64 values of codes [..., d / 2] and scale bytes [..., d / 32]."""
+    two = torch.stack((codes & 15, codes >> 4), dim=-1).flatten(-2).long()
+    value = torch.tensor(E2M1, dtype=torch.float64, device=codes.device)[two % 8]
+    value = torch.where(two >= 8, -value, value).unflatten(-1, (-1, 32))
+    scale = torch.where(scales == 255, float("nan"), torch.exp2(scales.double() - 127.0))
+    return (value * scale[..., None]).flatten(-2)
+
+
+@torch.no_grad()
+def rope_append_mxfp4(q: Tensor, k: Tensor, v: Tensor, cos: Tensor, sin: Tensor, positions: Tensor, slots: Tensor,
+                      k_codes: Tensor, k_scales: Tensor, v_codes: Tensor, v_scales: Tensor,
+                      interleaved: bool = False) -> tuple[Tensor, Tensor, Tensor]:
+    """As `rope_append`, the keys (rotated in float64) and values held as MXFP4 and returned as what that stands for."""
+    yq = _at_positions(q, cos, sin, positions, interleaved)
+    rows = _at_positions(k.double(), cos.double(), sin.double(), positions, interleaved), v.double()
+    kept, page, row = _cache_rows(slots, k_codes.shape[0], k_codes.shape[2])
+    held = []
+    for y, codes, scales in zip(rows, (k_codes, v_codes), (k_scales, v_scales)):
+        c, s = mxfp4_encode(y)
+        held.append(mxfp4_decode(c, s).to(k.dtype))
+        codes[page, :, row] = c[kept]
+        scales[page, :, :, row] = s[kept]
+    return yq, held[0], held[1]
+
+
+def _attend(q: Tensor, k: Tensor, v: Tensor, limits: Tensor, there: Tensor, scale: float) -> Tensor:
+    """q [n, hq, d] over k, v [L, hkv, d] (>= fp32): token t sees the keys below limits[t] that are `there`."""
+    group = q.shape[1] // k.shape[1]
+    seen = (torch.arange(k.shape[0], device=q.device) < limits[:, None]) & there
+    out = torch.zeros(q.shape, dtype=k.dtype, device=q.device)
+    for t in range(q.shape[0]):
+        at = torch.nonzero(seen[t])[:, 0]
+        if at.numel() == 0:
+            continue
+        kt = k[at].repeat_interleave(group, dim=1)
+        vt = v[at].repeat_interleave(group, dim=1)
+        p = torch.softmax((q[t].to(k.dtype) * kt).sum(-1) * scale, dim=0)
+        out[t] = (p[..., None] * vt).sum(0)
+    return out
+
+
+def _attn_paged(q, block_table, cache_lens, cu_seqlens, causal, softmax_scale, page_size: int, pages: int, kv_heads: int,
+                read) -> Tensor:
+    seqs = cache_lens.numel()
+    cuts = list(range(seqs + 1)) if cu_seqlens is None else cu_seqlens.tolist()
+    scale = q.shape[-1] ** -0.5 if softmax_scale is None else softmax_scale
+    o = torch.zeros_like(q)
+    for i, length in enumerate(cache_lens.tolist()):
+        first, last = cuts[i], cuts[i + 1]
+        key = torch.arange(min(max(length, 0), block_table.shape[1] * page_size), device=q.device)
+        page = block_table[i].long()[torch.div(key, page_size, rounding_mode="floor")]
+        there = (page >= 0) & (page < pages)
+        if last == first or not bool(there.any()):
+            continue
+        k, v = read(torch.where(there, page, 0), key % page_size)
+        n = last - first
+        limits = key.numel() - n + 1 + torch.arange(n, device=q.device) if causal else torch.full(
+            (n,), key.numel(), device=q.device)
+        o[first:last] = _attend(q[first:last], k, v, limits, there, scale).to(q.dtype)
+    return o
+
+
+def attn_paged(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, cache_lens: Tensor,
+               cu_seqlens: Tensor | None = None, causal: bool = True, softmax_scale: float | None = None) -> Tensor:
+    """softmax(q k^T scale) v of each sequence's new tokens over its cached keys, in >= fp32, rounded once."""
+    def read(page, row):
+        return upcast(k_cache[page, :, row]), upcast(v_cache[page, :, row])
+
+    return _attn_paged(q, block_table, cache_lens, cu_seqlens, causal, softmax_scale, k_cache.shape[2],
+                       k_cache.shape[0], k_cache.shape[1], read)
+
+
+def attn_paged_mxfp4(q: Tensor, k_codes: Tensor, k_scales: Tensor, v_codes: Tensor, v_scales: Tensor,
+                     block_table: Tensor, cache_lens: Tensor, cu_seqlens: Tensor | None = None, causal: bool = True,
+                     softmax_scale: float | None = None) -> Tensor:
+    """`attn_paged` over what an MXFP4 cache stands for."""
+    dtype = torch.promote_types(q.dtype, torch.float32)
+
+    def read(page, row):
+        return tuple(mxfp4_decode(c[page, :, row], s[page, :, :, row]).to(dtype)
+                     for c, s in ((k_codes, k_scales), (v_codes, v_scales)))
+
+    return _attn_paged(q, block_table, cache_lens, cu_seqlens, causal, softmax_scale, k_codes.shape[2],
+                       k_codes.shape[0], k_codes.shape[1], read)
+
+
+def distinct_slots(t: Tensor, dims, generator: torch.Generator) -> Tensor:
+    """Test-input transform: a different cache row for every token, the last token left out."""
+    pool = dims["pages"] * dims["page_size"]
+    if pool < t.numel():
+        raise ValueError(f"{t.numel()} tokens do not fit {pool} cache rows")
+    slots = torch.randperm(pool, generator=generator)[: t.numel()]
+    if t.numel() > 1:
+        slots[-1] = -1
+    return slots
+
+
+def cached_lengths(t: Tensor, dims, generator: torch.Generator) -> Tensor:
+    """Test-input transform: between 1 key and the table's capacity for every sequence."""
+    return torch.randint(1, dims["table_pages"] * dims["page_size"] + 1, t.shape, generator=generator).int()
+
+
+def table_entries(t: Tensor, dims, generator: torch.Generator) -> Tensor:
+    """Test-input transform: pages of the pool."""
+    return torch.randint(0, dims["pages"], t.shape, generator=generator).int()

@@ -78,6 +78,8 @@ BFloat16 = _Family("BFloat16", ("bfloat16",))
 Float32 = _Family("Float32", ("float32",))
 Float64 = _Family("Float64", ("float64",))
 Int32 = _Family("Int32", ("int32",))
+Int = _Family("Int", ("int32", "int64"))
+UInt8 = _Family("UInt8", ("uint8",))
 
 Token = typing.Union[str, int, "types.EllipsisType"]
 

@@ -33,6 +33,7 @@
 #include <cmath>
 #include <optional>
 #include <string>
+#include <vector>
 
 #include "../../include/popcorn_amd.h"
 
@@ -63,17 +64,20 @@ bool is_half(ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
 bool is_float(ScalarType t) { return t == at::kFloat || is_half(t); }
 ScalarType promoted(ScalarType a, ScalarType b) { return a == b ? a : at::kFloat; }  // of the three types above
 
-// A plain strided HIP tensor of a float type: no subclass behaviour, wrapper,
-// pending negation or tangent that reading its memory would miss.
-bool plain(const Tensor& t) {
+// A plain strided HIP tensor: no subclass behaviour, wrapper, pending negation or
+// tangent that reading its memory would miss.
+bool plain_memory(const Tensor& t) {
   const auto keys = t.key_set();
   static constexpr c10::DispatchKeySet other({c10::DispatchKey::Python, c10::DispatchKey::PythonTLSSnapshot,
                                               c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
                                               c10::DispatchKey::Functionalize, c10::DispatchKey::Negative,
                                               c10::DispatchKey::Conjugate, c10::DispatchKey::ZeroTensor});
   return keys.has(c10::DispatchKey::CUDA) && !keys.has_any(other) && t.layout() == at::kStrided && t.has_storage() &&
-         is_float(t.scalar_type()) && t.numel() > 0 && !t._fw_grad(0).defined();
+         t.numel() > 0 && !t._fw_grad(0).defined();
 }
+
+// One of a float type.
+bool plain(const Tensor& t) { return is_float(t.scalar_type()) && plain_memory(t); }
 
 // Whether a torch function mode is active that could look at the torch calls
 // inside one of these. The one behind torch.set_default_device and `with
@@ -99,6 +103,13 @@ bool take(PyObject* o, Tensor& t, const Tensor* like = nullptr) {
   if (!THPVariable_CheckExact(o)) return false;
   t = THPVariable_Unpack(o);
   return plain(t) && (like == nullptr || t.device() == like->device());
+}
+
+// The same of an integer type.
+bool take_whole(PyObject* o, Tensor& t, const Tensor& like, ScalarType type) {
+  if (!THPVariable_CheckExact(o)) return false;
+  t = THPVariable_Unpack(o);
+  return t.scalar_type() == type && plain_memory(t) && t.device() == like.device();
 }
 
 bool aligned(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0; }
@@ -694,6 +705,179 @@ PyObject* py_attn_varlen(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------- the paged cache
+
+// Two caches [pages, kv_heads, page_size, row] of one shape, rows contiguous.
+bool cache_pair(const Tensor& a, const Tensor& b, int64_t kv_heads, int64_t row) {
+  return a.dim() == 4 && a.sizes() == b.sizes() && a.size(1) == kv_heads && a.size(2) % 16 == 0 && a.size(3) == row &&
+         last_contiguous(a) && last_contiguous(b);
+}
+
+bool own_memory(const Tensor& t) {
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.stride(i) == 0 && t.size(i) > 1) return false;
+  return true;
+}
+
+// k's and v's cache: rows, or codes and then scales.
+struct Cache {
+  Tensor rows[2], scales[2];
+  bool mxfp4 = false;
+  // The next two (or four) arguments, for keys of `like`'s type.
+  bool take_from(PyObject* const* a, const Tensor& like, int64_t kv_heads, int64_t d) {
+    if (!mxfp4)
+      return take(a[0], rows[0], &like) && take(a[1], rows[1], &like) && rows[0].scalar_type() == like.scalar_type() &&
+             rows[1].scalar_type() == like.scalar_type() && cache_pair(rows[0], rows[1], kv_heads, d);
+    for (int i = 0; i < 2; ++i)
+      if (!take_whole(a[2 * i], rows[i], like, at::kByte) || !take_whole(a[2 * i + 1], scales[i], like, at::kByte)) return false;
+    if (d % 32 != 0 || !cache_pair(rows[0], rows[1], kv_heads, d / 2)) return false;
+    const int64_t want[4] = {rows[0].size(0), kv_heads, d / 32, rows[0].size(2)};
+    for (const Tensor& t : scales)
+      if (t.sizes() != at::IntArrayRef(want, 4) || !last_contiguous(t)) return false;
+    return true;
+  }
+  bool any_grad() const { return tracks({&rows[0], &rows[1]}); }
+};
+
+void lead(std::vector<int64_t>& st, const Tensor& t, int n) {
+  for (int i = 0; i < n; ++i) st.push_back(t.stride(i));
+}
+
+// q, k, v, cos, sin, positions, slots, the cache, interleaved
+PyObject* append(PyObject* const* a, Py_ssize_t n, bool mxfp4) {
+  Tensor q, k, v, cs, sn, at, to;
+  Cache c;
+  c.mxfp4 = mxfp4;
+  if (n != (mxfp4 ? 12 : 10) || watched() || !take(a[0], q) || !take(a[1], k, &q) || !take(a[2], v, &q) ||
+      !take(a[3], cs, &q) || !take(a[4], sn, &q) || !is_bool(a[n - 1]))
+    return decline();
+  if (q.dim() != 3 || k.dim() != 3 || k.sizes() != v.sizes() || q.size(0) != k.size(0) || q.size(2) != k.size(2) ||
+      q.scalar_type() != k.scalar_type() || q.scalar_type() != v.scalar_type() || !last_contiguous(q) ||
+      !last_contiguous(k) || !last_contiguous(v) || cs.dim() != 2 || cs.sizes() != sn.sizes() ||
+      cs.scalar_type() != sn.scalar_type() || !cs.is_contiguous() || !sn.is_contiguous() || 2 * cs.size(1) > q.size(2))
+    return decline();
+  const int64_t tokens = q.size(0), d = q.size(2), hkv = k.size(1);
+  const auto indices = [&](PyObject* o, Tensor& t) {
+    return (take_whole(o, t, q, at::kLong) || take_whole(o, t, q, at::kInt)) && t.dim() == 1 && t.size(0) == tokens &&
+           t.is_contiguous();
+  };
+  if (!indices(a[5], at) || !indices(a[6], to) || !c.take_from(a + 7, k, hkv, d) || tracks({&q, &k, &v, &cs, &sn}) ||
+      c.any_grad())
+    return decline();
+  for (int i = 0; i < 2; ++i)
+    if (!own_memory(c.rows[i]) || (mxfp4 && !own_memory(c.scales[i]))) return decline();
+  const bool interleaved = a[n - 1] == Py_True;
+  Tensor yq, yk, yv;
+  {
+    pybind11::gil_scoped_release free;
+    const c10::DeviceGuard guard(q.device());
+    const ScalarType dtype = q.scalar_type();
+    yq = empty(q.sizes(), dtype, q);
+    yk = empty(k.sizes(), dtype, q);
+    std::vector<int64_t> st;
+    st.reserve(18);
+    for (const Tensor* t : {&q, &k, &v}) lead(st, *t, 2);
+    for (const Tensor& t : c.rows) lead(st, t, 3);
+    const int wide_at = at.scalar_type() == at::kLong, wide_to = to.scalar_type() == at::kLong;
+    if (mxfp4) {
+      yv = empty(v.sizes(), dtype, q);
+      for (const Tensor& t : c.scales) lead(st, t, 3);
+      check(pk_rope_append_mxfp4(ptr(q), ptr(k), ptr(v), ptr(cs), ptr(sn), ptr(at), ptr(to), out(yq), out(yk), out(yv),
+                                 out(c.rows[0]), out(c.scales[0]), out(c.rows[1]), out(c.scales[1]), st.data(), tokens,
+                                 q.size(1), hkv, d, cs.size(1), cs.size(0), c.rows[0].size(0), c.rows[0].size(2),
+                                 code_of(dtype), code_of(cs.scalar_type()), wide_at, wide_to, interleaved, stream_of(q)));
+    } else {
+      check(pk_rope_append(ptr(q), ptr(k), ptr(v), ptr(cs), ptr(sn), ptr(at), ptr(to), out(yq), out(yk), out(c.rows[0]),
+                           out(c.rows[1]), st.data(), tokens, q.size(1), hkv, d, cs.size(1), cs.size(0),
+                           c.rows[0].size(0), c.rows[0].size(2), code_of(dtype), code_of(cs.scalar_type()), wide_at,
+                           wide_to, interleaved, stream_of(q)));
+    }
+  }
+  if (!mxfp4) return pair(std::move(yq), std::move(yk));
+  PyObject* t = PyTuple_New(3);
+  if (t == nullptr) return nullptr;
+  PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(std::move(yq)));
+  PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(std::move(yk)));
+  PyTuple_SET_ITEM(t, 2, THPVariable_Wrap(std::move(yv)));
+  return t;
+}
+
+PyObject* py_rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  return append(a, n, false);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_rope_append_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  return append(a, n, true);
+  END_HANDLE_TH_ERRORS
+}
+
+// q, the cache, block table, lengths, offsets or None, causal, scale
+PyObject* paged(PyObject* const* a, Py_ssize_t n, bool mxfp4) {
+  Tensor q, table, lens, cu;
+  Cache c;
+  c.mxfp4 = mxfp4;
+  double scale;
+  const int at = mxfp4 ? 5 : 3;
+  if (n != at + 5 || watched() || !take(a[0], q) || q.dim() != 3 || !THPVariable_CheckExact(a[1]) ||
+      THPVariable_Unpack(a[1]).dim() != 4)
+    return decline();
+  const int64_t total = q.size(0), hq = q.size(1), d = q.size(2), hkv = THPVariable_Unpack(a[1]).size(1);
+  if (hkv < 1 || hq % hkv != 0 || d % 8 != 0 || d > 256 || !aligned_rows(q) || !c.take_from(a + 1, q, hkv, d) ||
+      !take_whole(a[at], table, q, at::kInt) || !take_whole(a[at + 1], lens, q, at::kInt) || !is_bool(a[at + 3]) ||
+      !take_scale(a[at + 4], d, scale) || tracks({&q}) || c.any_grad())
+    return decline();
+  if (a[at + 2] != Py_None && (!take_whole(a[at + 2], cu, q, at::kInt) || cu.dim() != 1 || !cu.is_contiguous()))
+    return decline();
+  const int64_t seqs = cu.defined() ? cu.numel() - 1 : total;
+  if (table.dim() != 2 || table.size(0) != seqs || !last_contiguous(table) || lens.dim() != 1 || lens.size(0) != seqs ||
+      !lens.is_contiguous())
+    return decline();
+  const bool causal = a[at + 3] == Py_True;
+  Tensor o;
+  {
+    pybind11::gil_scoped_release free;
+    const c10::DeviceGuard guard(q.device());
+    o = empty(q.sizes(), q.scalar_type(), q);
+    const int code = code_of(q.scalar_type());
+    const int64_t pages = c.rows[0].size(0), page_size = c.rows[0].size(2), width = table.size(1);
+    const int64_t bytes =
+        pk_attn_paged_workspace(seqs, total, cu.defined(), hq, hkv, d, width * page_size, code, mxfp4);
+    Tensor ws;
+    if (bytes > 0) ws = scratch(bytes, q);
+    std::vector<int64_t> st;
+    st.reserve(14);
+    lead(st, q, 2);
+    for (const Tensor& t : c.rows) lead(st, t, 3);
+    const auto ints = [](const Tensor& t) { return static_cast<const int*>(ptr(t)); };
+    if (mxfp4) {
+      for (const Tensor& t : c.scales) lead(st, t, 3);
+      check(pk_attn_paged_mxfp4(ptr(q), ptr(c.rows[0]), ptr(c.scales[0]), ptr(c.rows[1]), ptr(c.scales[1]), ints(table),
+                                ints(lens), ints(cu), out(o), out(ws), bytes, st.data(), seqs, total, hq, hkv, d, pages,
+                                page_size, width, table.stride(0), (float)scale, causal, code, stream_of(q)));
+    } else {
+      check(pk_attn_paged(ptr(q), ptr(c.rows[0]), ptr(c.rows[1]), ints(table), ints(lens), ints(cu), out(o), out(ws),
+                          bytes, st.data(), seqs, total, hq, hkv, d, pages, page_size, width, table.stride(0),
+                          (float)scale, causal, code, stream_of(q)));
+    }
+  }
+  return THPVariable_Wrap(std::move(o));
+}
+
+PyObject* py_attn_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  return paged(a, n, false);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_attn_paged_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  return paged(a, n, true);
+  END_HANDLE_TH_ERRORS
+}
+
 // The exception to raise, and torch's mode of a default device.
 PyObject* py_set_types(PyObject*, PyObject* args) {
   PyObject *error, *context;
@@ -710,6 +894,8 @@ PyMethodDef methods[] = {
     PK_FAST("rms_norm", py_rms_norm),         PK_FAST("add_rms_norm", py_add_rms_norm), PK_FAST("swiglu", py_swiglu),
     PK_FAST("rotary_embedding", py_rotary),   PK_FAST("rope", py_rope),                 PK_FAST("qk_norm_rope", py_qk_norm_rope),
     PK_FAST("attn", py_attn),                 PK_FAST("attn_varlen", py_attn_varlen),
+    PK_FAST("rope_append", py_rope_append),   PK_FAST("rope_append_mxfp4", py_rope_append_mxfp4),
+    PK_FAST("attn_paged", py_attn_paged),     PK_FAST("attn_paged_mxfp4", py_attn_paged_mxfp4),
     {"set_types", py_set_types, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "popcorn_amd._native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -22,6 +22,16 @@ need a copy, empty tensors, and whatever has to be refused) is done here.
     attn(q, k, v, causal=False, softmax_scale=None) kernels/attn.py:10-37
     attn_varlen(q, k, v, cu_seqlens, causal=False, softmax_scale=None)
                                                     kernels/attn_varlen.py:15-54
+
+and, for answering token by token, a paged cache of keys and values (no counterpart
+in the reference; beside `rope` and `attn_varlen`, with references of their own in
+`popcorn_amd.compat`):
+
+    rope_append(q, k, v, cos, sin, positions, slots, k_cache, v_cache, interleaved=False)
+    rope_append_mxfp4(q, k, v, cos, sin, positions, slots, k_codes, k_scales, v_codes, v_scales, interleaved=False)
+    attn_paged(q, k_cache, v_cache, block_table, cache_lens, cu_seqlens=None, causal=True, softmax_scale=None)
+    attn_paged_mxfp4(q, k_codes, k_scales, v_codes, v_scales, block_table, cache_lens, cu_seqlens=None, causal=True,
+                     softmax_scale=None)
 """
 
 from __future__ import annotations
@@ -35,7 +45,7 @@ _compiling = torch.compiler.is_compiling  # a traced call stays in Python, where
 
 __all__ = ["rms_norm", "add_rms_norm", "swiglu", "rotary_embedding", "attn", "attn_with_lse", "attn_varlen",
            "attn_varlen_with_lse", "rotary_embedding_", "rope",
-           "qk_norm_rope"]
+           "qk_norm_rope", "rope_append", "rope_append_mxfp4", "attn_paged", "attn_paged_mxfp4"]
 
 
 def _require_cuda(*tensors: Tensor | None) -> torch.device:
@@ -885,3 +895,218 @@ class _AttentionVarlen(torch.autograd.Function):
                 lib,
             )
         return dq, dk, dv, None, None, None, None, None
+
+
+# --------------------------------------------------------------------------- paged cache
+
+
+def _no_gradient(name: str, *tensors: Tensor | None) -> None:
+    if _tracks_grad(*tensors):
+        raise RuntimeError(f"popcorn_amd.{name}: a cache has no gradient; call it under torch.no_grad() or on "
+                           "detached tensors")
+
+
+def _cache_rows(name: str, kv_heads: int, head_dim: int, unit: int, *caches: Tensor) -> tuple[int, int]:
+    """(pages, page size) of caches [pages, kv_heads, page_size, head_dim / unit]."""
+    shape = tuple(caches[0].shape)
+    if any(tuple(t.shape) != shape for t in caches) or len(shape) != 4 or shape[1] != kv_heads or (
+            shape[3] * unit != head_dim):
+        raise ValueError(f"popcorn_amd.{name}: caches {[tuple(t.shape) for t in caches]} must be [pages, {kv_heads}, "
+                         f"page_size, {head_dim // unit}]")
+    if any(t.stride(-1) != 1 for t in caches):
+        raise ValueError(f"popcorn_amd.{name}: the last dimension of a cache must be contiguous")
+    if shape[2] < 16 or shape[2] % 16:
+        raise ValueError(f"popcorn_amd.{name}: page_size={shape[2]} is not a multiple of 16")
+    return shape[0], shape[2]
+
+
+def _mxfp4_cache(name: str, kv_heads: int, head_dim: int, codes: tuple[Tensor, Tensor],
+                 scales: tuple[Tensor, Tensor]) -> tuple[int, int]:
+    if any(t.dtype != torch.uint8 for t in codes + scales):
+        raise TypeError(f"popcorn_amd.{name}: codes and scales must be uint8")
+    if head_dim % 32:
+        raise ValueError(f"popcorn_amd.{name}: head_dim={head_dim} is not a multiple of 32")
+    pages, page_size = _cache_rows(name, kv_heads, head_dim, 2, *codes)
+    want = (pages, kv_heads, head_dim // 32, page_size)
+    if any(tuple(t.shape) != want for t in scales) or any(t.stride(-1) != 1 for t in scales):
+        raise ValueError(f"popcorn_amd.{name}: scales {[tuple(t.shape) for t in scales]} must be {want}, the last "
+                         "dimension contiguous")
+    return pages, page_size
+
+
+def _append(name: str, q, k, v, cos, sin, positions, slots, interleaved, caches: tuple[Tensor, ...], mxfp4: bool):
+    """One launch: the checks of both append ops, their outputs and the call."""
+    device = _require_cuda(q, k, v, cos, sin, positions, slots, *caches)
+    _no_gradient(name, q, k, v, cos, sin, *caches)
+    dtype = _same_dtype(name, q, k, v)
+    cs_dtype = _table_dtype(name, cos, sin)
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+        raise ValueError(f"popcorn_amd.{name}: q [tokens, hq, d] and k, v [tokens, hkv, d] expected, got "
+                         f"{[tuple(t.shape) for t in (q, k, v)]}")
+    tokens, q_heads, head_dim = q.shape
+    kv_heads = k.shape[1]
+    if cos.dim() != 2 or cos.shape != sin.shape or not 1 <= cos.shape[1] <= head_dim // 2:
+        raise ValueError(f"popcorn_amd.{name}: cos/sin {tuple(cos.shape)} must be [positions, 1 to {head_dim // 2}]")
+    for what, t in (("positions", positions), ("slots", slots)):
+        if t.dtype not in (torch.int32, torch.int64) or tuple(t.shape) != (tokens,):
+            raise ValueError(f"popcorn_amd.{name}: {what} must be int32 or int64 [{tokens}]")
+    if mxfp4:
+        pages, page_size = _mxfp4_cache(name, kv_heads, head_dim, caches[0::2], caches[1::2])
+    else:
+        pages, page_size = _cache_rows(name, kv_heads, head_dim, 1, *caches)
+        if any(t.dtype != dtype for t in caches):
+            raise TypeError(f"popcorn_amd.{name}: a cache of {caches[0].dtype} beside keys of {dtype}")
+    if any(stride == 0 and size > 1 for t in caches for size, stride in zip(t.shape, t.stride())):
+        raise ValueError(f"popcorn_amd.{name}: a cache's rows share memory")
+    q_, k_, v_ = (_last_contiguous(t.detach()) for t in (q, k, v))
+    cs, sn, at, to = (t.detach().contiguous() for t in (cos, sin, positions, slots))
+    outs = [torch.empty(t.shape, dtype=dtype, device=device) for t in ((q, k, v) if mxfp4 else (q, k))]
+    rows = caches[0::2] if mxfp4 else caches
+    strides = [s for t in (q_, k_, v_) for s in t.stride()[:2]] + [s for t in rows for s in t.stride()[:3]]
+    if mxfp4:
+        strides += [s for t in caches[1::2] for s in t.stride()[:3]]
+    lib = _lib.load()
+    call = lib.pk_rope_append_mxfp4 if mxfp4 else lib.pk_rope_append
+    with _lib.on_device(device):
+        _lib.check(
+            call(
+                q_.data_ptr(), k_.data_ptr(), v_.data_ptr(), cs.data_ptr(), sn.data_ptr(), at.data_ptr(), to.data_ptr(),
+                *(t.data_ptr() for t in outs), *(t.data_ptr() for t in caches),
+                (_lib._i64 * len(strides))(*strides), tokens, q_heads, kv_heads, head_dim, cos.shape[1], cos.shape[0],
+                pages, page_size, _lib.dtype_code(dtype), _lib.dtype_code(cs_dtype), int(at.dtype == torch.int64),
+                int(to.dtype == torch.int64), int(bool(interleaved)), _lib.stream_handle(device),
+            ),
+            lib,
+        )
+    return tuple(outs)
+
+
+def rope_append(q: Tensor, k: Tensor, v: Tensor, cos: Tensor, sin: Tensor, positions: Tensor, slots: Tensor,
+                k_cache: Tensor, v_cache: Tensor, interleaved: bool = False) -> tuple[Tensor, Tensor]:
+    """Rotate new tokens' queries and keys and append their keys and values to a paged cache: (yq, yk).
+
+    q [tokens, q_heads, head_dim], k, v [tokens, kv_heads, head_dim]; cos, sin
+    [max_positions, half], read at `positions` [tokens] (clamped to the table); pairs and
+    arithmetic as `rotary_embedding`. k_cache, v_cache [pages, kv_heads, page_size,
+    head_dim] of k's type are written at `slots` [tokens]: row slot % page_size of page
+    slot // page_size. A slot below 0, or past the pool, is not written; two tokens must
+    not have the same one. One launch; no gradient.
+    """
+    if not _compiling():
+        ys = _lib.native().rope_append(q, k, v, cos, sin, positions, slots, k_cache, v_cache, interleaved)
+        if ys is not NotImplemented:
+            return ys
+    return _append("rope_append", q, k, v, cos, sin, positions, slots, interleaved, (k_cache, v_cache), False)
+
+
+def rope_append_mxfp4(q: Tensor, k: Tensor, v: Tensor, cos: Tensor, sin: Tensor, positions: Tensor, slots: Tensor,
+                      k_codes: Tensor, k_scales: Tensor, v_codes: Tensor, v_scales: Tensor,
+                      interleaved: bool = False) -> tuple[Tensor, Tensor, Tensor]:
+    """`rope_append` into a cache held as MXFP4: (yq, yk, yv), yk and yv being what the cache now stands for.
+
+    codes uint8 [pages, kv_heads, page_size, head_dim / 2] (two e2m1 codes, the even
+    channel low), scales uint8 [pages, kv_heads, head_dim / 32, page_size] (E8M0). yk and
+    yv have k's type: a prompt attended with them (`attn_varlen`) sees the keys and values
+    that its answer will see in the cache.
+    """
+    if not _compiling():
+        ys = _lib.native().rope_append_mxfp4(q, k, v, cos, sin, positions, slots, k_codes, k_scales, v_codes, v_scales,
+                                             interleaved)
+        if ys is not NotImplemented:
+            return ys
+    return _append("rope_append_mxfp4", q, k, v, cos, sin, positions, slots, interleaved,
+                   (k_codes, k_scales, v_codes, v_scales), True)
+
+
+def _attn_paged(name: str, q, block_table, cache_lens, cu_seqlens, causal, softmax_scale, caches: tuple[Tensor, ...],
+                mxfp4: bool) -> Tensor:
+    device = _require_cuda(q, block_table, cache_lens, cu_seqlens, *caches)
+    _no_gradient(name, q, *caches)
+    dtype = q.dtype
+    code = _lib.dtype_code(dtype)
+    if q.dim() != 3 or caches[0].dim() != 4:
+        raise ValueError(f"popcorn_amd.{name}: q [tokens, q_heads, head_dim] and a cache of four dimensions expected, got "
+                         f"{tuple(q.shape)} and {tuple(caches[0].shape)}")
+    total, q_heads, head_dim = q.shape
+    kv_heads = caches[0].shape[1]
+    if kv_heads == 0 or q_heads % kv_heads:
+        raise ValueError(f"popcorn_amd.{name}: q_heads={q_heads} is not a multiple of kv_heads={kv_heads}")
+    if mxfp4:
+        pages, page_size = _mxfp4_cache(name, kv_heads, head_dim, caches[0::2], caches[1::2])
+    else:
+        pages, page_size = _cache_rows(name, kv_heads, head_dim, 1, *caches)
+        if any(t.dtype != dtype for t in caches):
+            raise TypeError(f"popcorn_amd.{name}: a cache of {caches[0].dtype} beside queries of {dtype}")
+    given = [t for t in (block_table, cache_lens, cu_seqlens) if t is not None]
+    if any(t.dtype != torch.int32 for t in given):
+        raise TypeError(f"popcorn_amd.{name}: block_table, cache_lens and cu_seqlens must be int32")
+    seqs = total if cu_seqlens is None else cu_seqlens.numel() - 1
+    if (block_table.dim() != 2 or block_table.shape[0] != seqs or tuple(cache_lens.shape) != (seqs,)
+            or (cu_seqlens is not None and (cu_seqlens.dim() != 1 or seqs < 0))):
+        raise ValueError(f"popcorn_amd.{name}: block_table [{seqs}, pages], cache_lens [{seqs}] and cu_seqlens "
+                         f"[sequences + 1] expected, got {[tuple(t.shape) for t in given]}")
+    q_ = _aligned_rows(q.detach())
+    table = block_table if block_table.stride(-1) == 1 or block_table.shape[1] == 0 else block_table.contiguous()
+    lens = cache_lens.contiguous()
+    cu = None if cu_seqlens is None else cu_seqlens.contiguous()
+    o = torch.empty((total, q_heads, head_dim), dtype=dtype, device=device)
+    lib = _lib.load()
+    rows = caches[0::2] if mxfp4 else caches
+    strides = [*q_.stride()[:2], *(s for t in rows for s in t.stride()[:3])]
+    if mxfp4:
+        strides += [s for t in caches[1::2] for s in t.stride()[:3]]
+    with _lib.on_device(device):
+        nbytes = lib.pk_attn_paged_workspace(seqs, total, int(cu is not None), q_heads, kv_heads, head_dim,
+                                             table.shape[1] * page_size, code, int(mxfp4))
+        if nbytes < 0:
+            raise _lib.KernelError(f"popcorn_amd: pk_attn_paged_workspace: invalid shape {tuple(q.shape)}")
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        _lib.check(
+            (lib.pk_attn_paged_mxfp4 if mxfp4 else lib.pk_attn_paged)(
+                q_.data_ptr(), *(t.data_ptr() for t in caches), table.data_ptr(), lens.data_ptr(),
+                None if cu is None else cu.data_ptr(), o.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
+                (_lib._i64 * len(strides))(*strides), seqs, total, q_heads, kv_heads, head_dim, pages, page_size,
+                table.shape[1], table.stride(0), _scale(head_dim, softmax_scale), int(bool(causal)), code,
+                _lib.stream_handle(device),
+            ),
+            lib,
+        )
+    return o
+
+
+def attn_paged(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, cache_lens: Tensor,
+               cu_seqlens: Tensor | None = None, causal: bool = True, softmax_scale: float | None = None) -> Tensor:
+    """Attention of new tokens over a paged cache that holds their own keys and values too.
+
+    q [tokens, q_heads, head_dim]: one token a sequence, or packed runs of them with
+    cu_seqlens [sequences + 1] (int32). Sequence i has the first cache_lens[i] keys of the
+    pages block_table[i] (both int32); the last of its new tokens is the last key, and when
+    causal each attends the keys up to its own. k_cache, v_cache [pages, kv_heads,
+    page_size, head_dim] of q's type, page_size a multiple of 16, rows and pages a multiple
+    of 16 bytes apart; head_dim as for `attn`. A token without a key, or of no sequence,
+    gets zeros; keys on a page outside the pool are left out. Nothing is read back to the
+    host: a captured call may be replayed with other tables and lengths. No gradient.
+    Repeated calls give the same bits; how a sequence's keys are split follows the batch.
+    """
+    if not _compiling():
+        o = _lib.native().attn_paged(q, k_cache, v_cache, block_table, cache_lens, cu_seqlens, causal, softmax_scale)
+        if o is not NotImplemented:
+            return o
+    return _attn_paged("attn_paged", q, block_table, cache_lens, cu_seqlens, causal, softmax_scale, (k_cache, v_cache),
+                       False)
+
+
+def attn_paged_mxfp4(q: Tensor, k_codes: Tensor, k_scales: Tensor, v_codes: Tensor, v_scales: Tensor,
+                     block_table: Tensor, cache_lens: Tensor, cu_seqlens: Tensor | None = None, causal: bool = True,
+                     softmax_scale: float | None = None) -> Tensor:
+    """`attn_paged` over a cache held as MXFP4 (see `rope_append_mxfp4`), for q of any of the three types.
+
+    The cached values enter as they stand; q in fp16 or fp32 is not rounded to do so.
+    """
+    if not _compiling():
+        o = _lib.native().attn_paged_mxfp4(q, k_codes, k_scales, v_codes, v_scales, block_table, cache_lens, cu_seqlens,
+                                           causal, softmax_scale)
+        if o is not NotImplemented:
+            return o
+    return _attn_paged("attn_paged_mxfp4", q, block_table, cache_lens, cu_seqlens, causal, softmax_scale,
+                       (k_codes, k_scales, v_codes, v_scales), True)
