@@ -64,19 +64,21 @@ struct Args {
   const int* table;  // [seqs, width]
   const int* lens;   // [seqs]
   const int* cu;     // [seqs + 1], or NULL: one token a sequence
-  int64_t qt, qh;            // q strides, elements
-  int64_t kp, kh, vp, vh;    // page and head strides of the cache, bytes
-  int kt, vt;                // token strides, bytes
-  int64_t ksp, ksh, vsp, vsh;  // scales: page and head strides, bytes
-  int ksb, vsb;                // block strides
+  int64_t qt, qh;     // q strides, elements
+  int64_t page, head;  // page and head strides of both caches, bytes
+  int token;           // token stride
+  int64_t spage, shead;  // scales: page and head strides, bytes
+  int sblock;            // block stride
   int64_t table_stride;
   int width, pages, tiles_per_page;
+  int elem;  // bytes of a cached value (rows)
+  int tpp_shift, group_shift;  // log2 of tiles_per_page and group, or -1
   int seqs, total, heads, kv_heads, group, d;
   int causal;
   float c;  // scale * log2(e)
   int split;       // whether sequences may be split
   int min_chunk;   // keys
-  int64_t target;  // chunks a kv head
+  double per_chunk;  // 1 / the chunks a kv head is to have
   int items;       // blocks a kv head, and row tiles: what the workspace has room for, and offsets
   int tiles;       // that do not rise may ask for more
   // partial sums: part [items][kv_heads][rows][d], ml [items][kv_heads][rows][2], meta [1 + 4 * row tiles]
@@ -97,16 +99,23 @@ struct Seq {
 };
 
 __device__ __forceinline__ Seq seq_of(const Args& a, int i) {
-  Seq s;
+  Seq s = {i, 1, min(max(a.lens[i], 0), a.width * a.tiles_per_page * 16)};  // at most 2^30
   if (a.cu) {
     s.start = min(max(a.cu[i], 0), a.total);
     s.n = min(max(a.cu[i + 1], s.start), a.total) - s.start;
-  } else {
-    s.start = i;
-    s.n = 1;
   }
-  s.len = (int)min((int64_t)max(a.lens[i], 0), (int64_t)a.width * a.tiles_per_page * 16);
   return s;
+}
+
+// Token and head in the group of a row.
+__device__ __forceinline__ int token_of(const Args& a, int row) {
+  return a.group_shift >= 0 ? row >> a.group_shift : row / a.group;
+}
+
+// Output of a row of a sequence that starts at token `start`.
+template <typename T> __device__ __forceinline__ T* row_of(const Args& a, int start, int h, int row) {
+  const int token = token_of(a, row);
+  return static_cast<T*>(a.o) + ((int64_t)(start + token) * a.heads + h * a.group + row - token * a.group) * a.d;
 }
 
 struct Item {
@@ -125,28 +134,33 @@ template <int ROWS> __device__ __forceinline__ Item find(const Args& a, int x) {
   it.seq = -1;
   it.keys = 1 << 30;
   int tiles = 0;
+  Seq s = {0, 0, 0};
   if (a.split) {
     int64_t work = 0;
     for (int i = lane; i < a.seqs; i += 64) {
-      const Seq s = seq_of(a, i);
-      const int rt = (int)(((int64_t)s.n * a.group + ROWS - 1) / ROWS);
+      s = seq_of(a, i);
+      const int rt = (int)(((unsigned)s.n * (unsigned)a.group + ROWS - 1) / ROWS);
       work += (int64_t)rt * s.len;
       tiles += rt;
     }
     work = wave_sum64(work);
-    tiles = (int)wave_sum64(tiles);
-    const int64_t even = (work + a.target - 1) / a.target;
-    it.keys = (int)min(max((even + 63) / 64 * 64, (int64_t)a.min_chunk), (int64_t)1 << 30);
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) tiles += __shfl_xor(tiles, off, 64);
+    tiles = __builtin_amdgcn_readfirstlane(tiles);
+    // one more than the quotient: never fewer keys than an even share
+    const int even = (int)fmin((double)work * a.per_chunk, 1073741000.0) + 1;
+    it.keys = __builtin_amdgcn_readfirstlane(max((even + 63) / 64 * 64, a.min_chunk));
   }
   it.all_tiles = tiles;
-  int64_t before = 0;
-  int tiles_before = 0;
+  int before = 0, tiles_before = 0;
   for (int base = 0; base < a.seqs; base += 64) {
     const int i = base + lane;
-    Seq s = {0, 0, 0};
-    if (i < a.seqs) s = seq_of(a, i);
-    const int rt = (int)(((int64_t)s.n * a.group + ROWS - 1) / ROWS);
-    const int splits = max(1, (int)(((int64_t)s.len + it.keys - 1) / it.keys));
+    if (a.seqs > 64 || !a.split) {
+      s = Seq{0, 0, 0};
+      if (i < a.seqs) s = seq_of(a, i);
+    }
+    const int rt = (int)(((unsigned)s.n * (unsigned)a.group + ROWS - 1) / ROWS);
+    const int splits = a.split ? max(1, (int)(((unsigned)s.len + (unsigned)it.keys - 1) / (unsigned)it.keys)) : 1;
     const int mine = rt * splits;
     int upto = mine, rts = rt;  // inclusive sums over the lanes
 #pragma unroll
@@ -154,7 +168,7 @@ template <int ROWS> __device__ __forceinline__ Item find(const Args& a, int x) {
       const int p = __shfl_up(upto, off, 64), q = __shfl_up(rts, off, 64);
       if (lane >= off) upto += p, rts += q;
     }
-    const int64_t rel = x - before;
+    const int rel = x - before;
     const uint64_t found = __ballot(rel >= upto - mine && rel < upto);
     if (found != 0) {
       const int at = __builtin_ctzll(found);
@@ -163,9 +177,11 @@ template <int ROWS> __device__ __forceinline__ Item find(const Args& a, int x) {
       it.s.n = __builtin_amdgcn_readlane(s.n, at);
       it.s.len = __builtin_amdgcn_readlane(s.len, at);
       it.splits = __builtin_amdgcn_readlane(splits, at);
-      const int k = (int)(rel - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(mine, at)));
-      it.tile = k / it.splits;
-      it.chunk = k - it.tile * it.splits;
+      const int k = rel - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(mine, at));
+      const int tile = it.splits == 1 ? k : (int)((unsigned)k / (unsigned)it.splits);
+      it.chunk = k - tile * it.splits;
+      // the last row tiles see the most keys when causal: they go first
+      it.tile = __builtin_amdgcn_readlane(rt, at) - 1 - tile;
       it.tiles_base = tiles_before + __builtin_amdgcn_readlane(rts, at) - __builtin_amdgcn_readlane(rt, at);
       return it;
     }
@@ -181,14 +197,41 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const void* base, int 
 typedef unsigned w2 __attribute__((ext_vector_type(2)));
 typedef unsigned w4 __attribute__((ext_vector_type(4)));
 
-// One tile of 16 keys: where its rows lie, and how many of them are visible.
-struct Tile {
-  int page, off, rows;  // page < 0 or rows <= 0: nothing is read
+// The tiles of 16 keys of 64 / TILES steps, a lane each: where a tile's rows lie in the
+// cache (k and v alike) and how many bytes from there hold visible ones.
+struct Look {
+  uint64_t at, scales;  // byte offsets from the kv head's first row and scale
+  int bytes;            // 0: a page that is not there, or behind the last key
+  uint64_t whole, there;  // lanes whose tile has 16 visible keys, and any page
 };
 
-// bytes of `rows` rows of `width` bytes that lie `step` apart
-__device__ __forceinline__ int span(const Tile& t, int step, int width) {
-  return t.page < 0 || t.rows <= 0 ? 0 : (min(t.rows, 16) - 1) * step + width;
+// key: of this lane's tile; k1: the end of the visible ones
+template <bool MX> __device__ __forceinline__ Look look_up(const Args& a, int seq, int64_t key, int k1) {
+  Look l = {0, 0, 0, 0, 0};
+  int rows = 0;
+  if (key < k1) {
+    const int tile = (int)(key >> 4), slot = a.tpp_shift >= 0 ? tile >> a.tpp_shift : tile / a.tiles_per_page;
+    const int p = a.table[seq * a.table_stride + slot];
+    if (p >= 0 && p < a.pages) {
+      const int row = (tile - slot * a.tiles_per_page) * 16;
+      rows = min(k1 - (int)key, 16);
+      l.at = (uint64_t)p * a.page + (uint64_t)row * (unsigned)a.token;
+      l.bytes = (rows - 1) * a.token + (MX ? a.d / 2 : a.d * (int)a.elem);
+      if constexpr (MX) l.scales = (uint64_t)p * a.spage + row;
+    }
+  }
+  l.whole = __ballot(rows == 16);
+  l.there = __ballot(rows > 0);
+  return l;
+}
+
+__device__ __forceinline__ uint64_t lane64(uint64_t v, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, lane), hi = __builtin_amdgcn_readlane((uint32_t)(v >> 32), lane);
+  return ((uint64_t)hi << 32) | lo;
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const char* base, uint64_t at, int bytes, int lane) {
+  return rsrc_of(base + lane64(at, lane), __builtin_amdgcn_readlane(bytes, lane));
 }
 
 // A operand of eight 16-bit values from element e of eight rows, and of those with ones in m
@@ -220,9 +263,16 @@ template <> struct Mma16<f16> {
   }
 };
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
-  return (uint32_t)__builtin_bit_cast(uint16_t, from_f32<T>(a)) |
-         ((uint32_t)__builtin_bit_cast(uint16_t, from_f32<T>(b)) << 16);
+  typedef T pair __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, pair));
+}
+template <typename T> __device__ __forceinline__ f32x2 unpack2(uint32_t w) {
+  if constexpr (__is_same(T, bf16)) return {__builtin_bit_cast(float, w << 16), __builtin_bit_cast(float, w & 0xffff0000u)};
+  typedef T pair __attribute__((ext_vector_type(2)));
+  const pair p = __builtin_bit_cast(pair, w);
+  return {to_f32(p.x), to_f32(p.y)};
 }
 
 // The eight values x as TERMS operands of type T whose sum they are: rounded, then
@@ -234,7 +284,10 @@ template <typename T, int TERMS> __device__ __forceinline__ void terms_of(float 
     for (int w = 0; w < 4; ++w) out[t][w] = pack2<T>(x[2 * w], x[2 * w + 1]);
     if (t + 1 < TERMS) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] -= round_to<T>(x[i]);
+      for (int w = 0; w < 4; ++w) {
+        const f32x2 r = unpack2<T>(out[t][w]);
+        x[2 * w] -= r.x, x[2 * w + 1] -= r.y;
+      }
     }
   }
 }
@@ -275,28 +328,32 @@ __device__ __forceinline__ void add_if(bool in, const f32x4& x, f32x4& acc) {
   for (int c = 0; c < 4; ++c) acc[c] += in ? x[c] : 0.f;
 }
 
-// Rows of 16-bit values, of q's type.
+// Rows of 16-bit values, of q's type. P is two terms of it: one would add as much error
+// as rounding the output does, and the products are not what bounds a few rows.
 template <typename T_, int DL_> struct Rows16 {
   typedef T_ T;
-  static constexpr int DL = DL_, VL = DL / 16, SUB = 1, QN = DL / 32;
-  static constexpr int kWideR = 2;
+  static constexpr int DL = DL_, VL = DL / 16, SUB = 1, QN = DL / 32, VH = VL > 8 ? 2 : 1;
+  static constexpr bool kMx = false;
   struct Buf {
     w4 k[2][QN];
     uint32_t v[8][VL / 2];
   };
   typedef w4 Query[QN];
-  typedef w4 Prob;  // P of 32 keys
-  int koff[QN], voff[4][VL > 8 ? 2 : 1];
+  typedef w4 Prob[2];  // P of 32 keys
+  const char *kb, *vb;
+  int koff[QN], voff[4][VH];
 
-  __device__ __forceinline__ void init(const Args& a) {
+  __device__ __forceinline__ void init(const Args& a, int h) {
     const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
+    kb = static_cast<const char*>(a.k) + h * a.head;
+    vb = static_cast<const char*>(a.v) + h * a.head;
 #pragma unroll
-    for (int j = 0; j < QN; ++j) koff[j] = 32 * j + 8 * g < a.d ? n * a.kt + (32 * j + 8 * g) * 2 : kPad;
+    for (int j = 0; j < QN; ++j) koff[j] = 32 * j + 8 * g < a.d ? n * a.token + (32 * j + 8 * g) * 2 : kPad;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int h = 0; h < (VL > 8 ? 2 : 1); ++h)
-        voff[i][h] = VL * n + 8 * h < a.d ? (4 * g + i) * a.vt + (VL * n + 8 * h) * 2 : kPad;
+      for (int h = 0; h < VH; ++h)
+        voff[i][h] = VL * n + 8 * h < a.d ? (4 * g + i) * a.token + (VL * n + 8 * h) * 2 : kPad;
   }
   static __device__ __forceinline__ void query(const Args& a, const T* row, bool live, Query& q) {
     const int g = (threadIdx.x & 63) >> 4;
@@ -306,22 +363,18 @@ template <typename T_, int DL_> struct Rows16 {
       if (live && 32 * j + 8 * g < a.d) q[j] = *reinterpret_cast<const w4*>(row + 32 * j + 8 * g);
     }
   }
-  __device__ __forceinline__ void load_k(const Args& a, int h, const Tile (&t)[2], Buf& b) const {
+  __device__ __forceinline__ void load_k(const Look& l, int at, Buf& b) const {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int64_t page = max(t[u].page, 0);
-      const auto kr = rsrc_of(static_cast<const char*>(a.k) + page * a.kp + h * a.kh + (int64_t)t[u].off * a.kt,
-                              span(t[u], a.kt, a.d * 2));
+      const auto kr = tile_rsrc(kb, l.at, l.bytes, at + u);
 #pragma unroll
       for (int j = 0; j < QN; ++j) b.k[u][j] = __builtin_amdgcn_raw_buffer_load_b128(kr, koff[j], 0, 0);
     }
   }
-  __device__ __forceinline__ void load_v(const Args& a, int h, const Tile (&t)[2], Buf& b) const {
+  __device__ __forceinline__ void load_v(const Look& l, int at, Buf& b) const {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int64_t page = max(t[u].page, 0);
-      const auto vr = rsrc_of(static_cast<const char*>(a.v) + page * a.vp + h * a.vh + (int64_t)t[u].off * a.vt,
-                              span(t[u], a.vt, a.d * 2));
+      const auto vr = tile_rsrc(vb, l.at, l.bytes, at + u);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint32_t(&to)[VL / 2] = b.v[4 * u + i];
@@ -330,7 +383,7 @@ template <typename T_, int DL_> struct Rows16 {
           to[0] = x.x, to[1] = x.y;
         } else {
 #pragma unroll
-          for (int hh = 0; hh < VL / 8; ++hh) {
+          for (int hh = 0; hh < VH; ++hh) {
             const w4 x = __builtin_amdgcn_raw_buffer_load_b128(vr, voff[i][hh], 0, 0);
 #pragma unroll
             for (int w = 0; w < 4; ++w) to[4 * hh + w] = x[w];
@@ -340,16 +393,18 @@ template <typename T_, int DL_> struct Rows16 {
     }
   }
   // behind a sequence's last key everything reads as zero already
-  static __device__ __forceinline__ void trim(Buf&, const Tile (&)[2]) {}
+  static __device__ __forceinline__ void trim(Buf&, int) {}
   static __device__ __forceinline__ f32x4 score(const Buf& b, int t, const Query& q) {
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < QN; ++j) s = Mma16<T>::run(b.k[t][j], q[j], s);
     return s;
   }
-  // P, rounded to the values' type: the products' own
   static __device__ __forceinline__ void prob(const f32x4& lo, const f32x4& hi, Prob& p) {
-    p = w4{pack2<T>(lo[0], lo[1]), pack2<T>(lo[2], lo[3]), pack2<T>(hi[0], hi[1]), pack2<T>(hi[2], hi[3])};
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = lo[i], x[4 + i] = hi[i];
+    terms_of<T, 2>(x, p);
   }
   template <int R>
   static __device__ __forceinline__ void pv(const Buf& b, int, const Prob (&p)[R], f32x4 (&acc)[R][VL]) {
@@ -357,7 +412,9 @@ template <typename T_, int DL_> struct Rows16 {
     for (int e = 0; e < VL; ++e) {
       const w4 f = pick(b.v, e);
 #pragma unroll
-      for (int r = 0; r < R; ++r) acc[r][e] = Mma16<T>::run(f, p[r], acc[r][e]);
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) acc[r][e] = Mma16<T>::run(f, p[r][m], acc[r][e]);
     }
   }
   // The same product one key at a time, added to the rows that see it: in(r, key).
@@ -371,7 +428,12 @@ template <typename T_, int DL_> struct Rows16 {
       for (int e = 0; e < VL; ++e) {
         const w4 f = pick(b.v, e, mask);
 #pragma unroll
-        for (int r = 0; r < R; ++r) add_if(in(r, key), Mma16<T>::run(f, only(p[r], mask), f32x4{0.f, 0.f, 0.f, 0.f}), acc[r][e]);
+        for (int r = 0; r < R; ++r) {
+          f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int m = 0; m < 2; ++m) s = Mma16<T>::run(f, only(p[r][m], mask), s);
+          add_if(in(r, key), s, acc[r][e]);
+        }
       }
     }
   }
@@ -390,7 +452,6 @@ template <typename T_, int DL_> struct Rows16 {
 template <int DL_> struct Rows32 {
   typedef float T;
   static constexpr int DL = DL_, VL = DL / 16, SUB = 1, QN = DL / 16;
-  static constexpr int kWideR = DL <= 128 ? 2 : 1;
   struct Buf {
     f32x4 k[2][QN];
     f32x4 v[8][VL / 4];
@@ -399,16 +460,20 @@ template <int DL_> struct Rows32 {
   struct Prob {
     float p[8];
   };
+  static constexpr bool kMx = false;
+  const char *kb, *vb;
   int koff[QN], voff[4][VL / 4];
 
-  __device__ __forceinline__ void init(const Args& a) {
+  __device__ __forceinline__ void init(const Args& a, int h) {
     const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
+    kb = static_cast<const char*>(a.k) + h * a.head;
+    vb = static_cast<const char*>(a.v) + h * a.head;
 #pragma unroll
-    for (int j = 0; j < QN; ++j) koff[j] = 16 * j + 4 * g < a.d ? n * a.kt + (16 * j + 4 * g) * 4 : kPad;
+    for (int j = 0; j < QN; ++j) koff[j] = 16 * j + 4 * g < a.d ? n * a.token + (16 * j + 4 * g) * 4 : kPad;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int h = 0; h < VL / 4; ++h) voff[i][h] = VL * n + 4 * h < a.d ? (4 * g + i) * a.vt + (VL * n + 4 * h) * 4 : kPad;
+      for (int h = 0; h < VL / 4; ++h) voff[i][h] = VL * n + 4 * h < a.d ? (4 * g + i) * a.token + (VL * n + 4 * h) * 4 : kPad;
   }
   static __device__ __forceinline__ void query(const Args& a, const T* row, bool live, Query& q) {
     const int g = (threadIdx.x & 63) >> 4;
@@ -418,23 +483,19 @@ template <int DL_> struct Rows32 {
       if (live && 16 * j + 4 * g < a.d) q[j] = *reinterpret_cast<const f32x4*>(row + 16 * j + 4 * g);
     }
   }
-  __device__ __forceinline__ void load_k(const Args& a, int h, const Tile (&t)[2], Buf& b) const {
+  __device__ __forceinline__ void load_k(const Look& l, int at, Buf& b) const {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int64_t page = max(t[u].page, 0);
-      const auto kr = rsrc_of(static_cast<const char*>(a.k) + page * a.kp + h * a.kh + (int64_t)t[u].off * a.kt,
-                              span(t[u], a.kt, a.d * 4));
+      const auto kr = tile_rsrc(kb, l.at, l.bytes, at + u);
 #pragma unroll
       for (int j = 0; j < QN; ++j)
         b.k[u][j] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(kr, koff[j], 0, 0));
     }
   }
-  __device__ __forceinline__ void load_v(const Args& a, int h, const Tile (&t)[2], Buf& b) const {
+  __device__ __forceinline__ void load_v(const Look& l, int at, Buf& b) const {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int64_t page = max(t[u].page, 0);
-      const auto vr = rsrc_of(static_cast<const char*>(a.v) + page * a.vp + h * a.vh + (int64_t)t[u].off * a.vt,
-                              span(t[u], a.vt, a.d * 4));
+      const auto vr = tile_rsrc(vb, l.at, l.bytes, at + u);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -442,7 +503,7 @@ template <int DL_> struct Rows32 {
           b.v[4 * u + i][hh] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(vr, voff[i][hh], 0, 0));
     }
   }
-  static __device__ __forceinline__ void trim(Buf&, const Tile (&)[2]) {}
+  static __device__ __forceinline__ void trim(Buf&, int) {}
   static __device__ __forceinline__ f32x4 score(const Buf& b, int t, const Query& q) {
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -499,15 +560,15 @@ template <int DL_> struct Rows32 {
 // Rows of MXFP4 codes, 64 keys a step. A lane's K piece is DL / 4 consecutive
 // channels (16 bytes are one block of 32), a V piece VL, inside one block. They become
 // bf16, exactly, in registers; q and P are as many bf16 terms as their type has bits
-// for (bf16 one, fp16 two, fp32 three), so nothing is rounded but P of bf16.
+// for (bf16 one, fp16 two, fp32 three), and P of bf16 two as well, so nothing is rounded on the way.
 template <typename T_, int DL_> struct RowsMx {
   typedef T_ T;
   static constexpr int DL = DL_, VL = DL / 16, SUB = 2, QN = DL / 32;
-  static constexpr int TERMS = sizeof(T) == 4 ? 3 : (__is_same(T, bf16) ? 1 : 2);
+  static constexpr int TERMS = sizeof(T) == 4 ? 3 : (__is_same(T, bf16) ? 1 : 2), PTERMS = sizeof(T) == 4 ? 3 : 2;
+  static constexpr bool kMx = true;
   static constexpr int KW = DL >= 128 ? 4 : 2;     // words of codes in a K piece
   static constexpr int KP = DL >= 128 ? DL / 128 : 1;  // K pieces of a row in a lane
   static constexpr int VW = VL >= 8 ? VL / 8 : 1;  // words of codes of a V row in a lane (half a word at DL 64)
-  static constexpr int kWideR = 2;
   struct Buf {
     uint32_t k[4][KP][KW];
     uint32_t ke[4][KP];  // scale bytes
@@ -515,45 +576,52 @@ template <typename T_, int DL_> struct RowsMx {
     uint32_t ve[4];  // scale bytes of the lane's four keys of each tile
   };
   typedef w4 Query[QN][TERMS];
-  typedef w4 Prob[TERMS];
+  typedef w4 Prob[PTERMS];
+  const char *kb, *vb, *kse_b, *vse_b;
+  int scale_bytes;  // from a tile's first scale to behind its last
   int koff[KP], kse[KP], voff[4], vse;
 
   // channel of K piece word: product j takes these eight channels of a row from lane group g
   static __device__ __forceinline__ int channel(int j, int g) {
     return DL >= 128 ? 128 * (j / 4) + 32 * g + 8 * (j % 4) : 16 * g + 8 * j;
   }
-  __device__ __forceinline__ void init(const Args& a) {
+  __device__ __forceinline__ void init(const Args& a, int h) {
     const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
+    kb = static_cast<const char*>(a.k) + h * a.head;
+    vb = static_cast<const char*>(a.v) + h * a.head;
+    kse_b = reinterpret_cast<const char*>(a.ks) + h * a.shead;
+    vse_b = reinterpret_cast<const char*>(a.vs) + h * a.shead;
+    scale_bytes = (a.d / 32 - 1) * a.sblock + 16;
 #pragma unroll
     for (int p = 0; p < KP; ++p) {
       const int c = channel(4 * p, g);
-      koff[p] = c < a.d ? n * a.kt + c / 2 : kPad;
-      kse[p] = c < a.d ? (c / 32) * a.ksb + n : kPad;
+      koff[p] = c < a.d ? n * a.token + c / 2 : kPad;
+      kse[p] = c < a.d ? (c / 32) * a.sblock + n : kPad;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) voff[i] = VL * n < a.d ? (4 * g + i) * a.vt + VL * n / 2 : kPad;
-    vse = VL * n < a.d ? (VL * n / 32) * a.vsb + 4 * g : kPad;
+    for (int i = 0; i < 4; ++i) voff[i] = VL * n < a.d ? (4 * g + i) * a.token + VL * n / 2 : kPad;
+    vse = VL * n < a.d ? (VL * n / 32) * a.sblock + 4 * g : kPad;
   }
   static __device__ __forceinline__ void query(const Args& a, const T* row, bool live, Query& q) {
     const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
     for (int j = 0; j < QN; ++j) {
-      float x[8];
       const int c = channel(j, g);
+      Lane<T, 8> raw;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = live && c < a.d ? to_f32(row[c + i]) : 0.f;
+      for (int i = 0; i < Lane<T, 8>::kVectors; ++i) reinterpret_cast<w4*>(raw.v)[i] = w4{0, 0, 0, 0};
+      if (live && c < a.d) raw = ld_lane<T, 8>(row + c);
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = to_f32(raw.v[i]);
       terms_of<bf16, TERMS>(x, q[j]);
     }
   }
-  __device__ __forceinline__ void load_k(const Args& a, int h, const Tile (&t)[4], Buf& b) const {
-    const int blocks = a.d / 32;
+  __device__ __forceinline__ void load_k(const Look& l, int at, Buf& b) const {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int64_t page = max(t[u].page, 0);
-      const auto kr = rsrc_of(static_cast<const char*>(a.k) + page * a.kp + h * a.kh + (int64_t)t[u].off * a.kt,
-                              span(t[u], a.kt, a.d / 2));
-      const auto sr = rsrc_of(a.ks + page * a.ksp + h * a.ksh + t[u].off,
-                              t[u].page < 0 || t[u].rows <= 0 ? 0 : (blocks - 1) * a.ksb + 16);
+      const auto kr = paged::tile_rsrc(kb, l.at, l.bytes, at + u);
+      const auto sr = rsrc_of(kse_b + lane64(l.scales, at + u), (l.there >> (at + u)) & 1 ? scale_bytes : 0);
 #pragma unroll
       for (int p = 0; p < KP; ++p) {
         if constexpr (KW == 4) {
@@ -568,15 +636,11 @@ template <typename T_, int DL_> struct RowsMx {
       }
     }
   }
-  __device__ __forceinline__ void load_v(const Args& a, int h, const Tile (&t)[4], Buf& b) const {
-    const int blocks = a.d / 32;
+  __device__ __forceinline__ void load_v(const Look& l, int at, Buf& b) const {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int64_t page = max(t[u].page, 0);
-      const auto vr = rsrc_of(static_cast<const char*>(a.v) + page * a.vp + h * a.vh + (int64_t)t[u].off * a.vt,
-                              span(t[u], a.vt, a.d / 2));
-      const auto sr = rsrc_of(a.vs + page * a.vsp + h * a.vsh + t[u].off,
-                              t[u].page < 0 || t[u].rows <= 0 ? 0 : (blocks - 1) * a.vsb + 16);
+      const auto vr = paged::tile_rsrc(vb, l.at, l.bytes, at + u);
+      const auto sr = rsrc_of(vse_b + lane64(l.scales, at + u), (l.there >> (at + u)) & 1 ? scale_bytes : 0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint32_t(&to)[VW] = b.v[4 * u + i];
@@ -592,12 +656,13 @@ template <typename T_, int DL_> struct RowsMx {
       b.ve[u] = __builtin_amdgcn_raw_buffer_load_b32(sr, vse, 0, 0);
     }
   }
-  // The scales of keys behind the last one, whatever they are, as if their rows were zeros.
-  static __device__ __forceinline__ void trim(Buf& b, const Tile (&t)[4]) {
+  // The scales of keys behind the last one, whatever they are, as if their rows were
+  // zeros; `rows`: visible keys from the step's first on.
+  static __device__ __forceinline__ void trim(Buf& b, int rows) {
     const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int n = min(max(t[u].rows - 4 * g, 0), 4);
+      const int n = min(max(rows - 16 * u - 4 * g, 0), 4);
       b.ve[u] &= n == 4 ? 0xffffffffu : (1u << (8 * n)) - 1u;
     }
   }
@@ -616,7 +681,7 @@ template <typename T_, int DL_> struct RowsMx {
     float x[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = lo[i], x[4 + i] = hi[i];
-    terms_of<bf16, TERMS>(x, p);
+    terms_of<bf16, PTERMS>(x, p);
   }
   // The values of tiles 2 u and 2 u + 1 as bf16, VL to a row
   static __device__ __forceinline__ void decode(const Buf& b, int u, uint32_t (&v)[8][VL / 2]) {
@@ -647,7 +712,7 @@ template <typename T_, int DL_> struct RowsMx {
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int m = 0; m < TERMS; ++m) acc[r][e] = Mma16<bf16>::run(f, p[r][m], acc[r][e]);
+        for (int m = 0; m < PTERMS; ++m) acc[r][e] = Mma16<bf16>::run(f, p[r][m], acc[r][e]);
     }
   }
   template <int R, typename F>
@@ -665,7 +730,7 @@ template <typename T_, int DL_> struct RowsMx {
         for (int r = 0; r < R; ++r) {
           f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int m = 0; m < TERMS; ++m) s = Mma16<bf16>::run(f, only(p[r][m], mask), s);
+          for (int m = 0; m < PTERMS; ++m) s = Mma16<bf16>::run(f, only(p[r][m], mask), s);
           add_if(in(r, key), s, acc[r][e]);
         }
       }
@@ -681,7 +746,28 @@ template <typename T_, int DL_> struct RowsMx {
   }
 };
 
-// ---------------------------------------------------------------- the kernel
+// Zeros for the tokens that no sequence holds.
+template <typename T> __device__ __forceinline__ void zero_others(const Args& a) {
+  if (!a.cu) return;
+  const int first = min(max(a.cu[0], 0), a.total), last = min(max(a.cu[a.seqs], first), a.total);
+  for (int64_t i = blockIdx.x; i < first + a.total - last; i += gridDim.x) {
+    T* row = static_cast<T*>(a.o) + (i < first ? i : i - first + last) * (int64_t)a.heads * a.d;
+    for (int j = threadIdx.x; j < a.heads * a.d; j += kThreads) row[j] = from_f32<T>(0.f);
+  }
+}
+
+// What the joining kernel reads: the row tiles there are, and of a tile of more than one
+// chunk its first block and its rows.
+__device__ __forceinline__ void note(const Args& a, const Item& it, int x, int h, int row0, int rows) {
+  if (!a.split || h != 0 || it.chunk != 0 || threadIdx.x != 0 || it.tiles_base + it.tile >= a.tiles) return;
+  int* m = a.meta + 1 + 4 * (int64_t)(it.tiles_base + it.tile);
+  m[0] = x;
+  m[1] = it.splits;
+  m[2] = it.s.start * a.group + row0;  // the tile's first row among all rows of a kv head
+  m[3] = rows;
+}
+
+// ---------------------------------------------------------------- the kernel of few rows
 
 // SPLIT: the block's waves hold the same 16 R rows and take the steps of the chunk in
 // turn, their sums joined in LDS at the end. Otherwise each wave has 16 R rows of its
@@ -691,14 +777,14 @@ template <class C, int R, bool SPLIT> struct Shape {
 };
 
 // Waves a SIMD holds: what the registers of a step's rows allow.
-template <class C, int R> constexpr int kWavesPerEu = (C::DL / 128 + 1) * (sizeof(typename C::Buf) / 128 + R) > 8 ? 1 : 2;
+template <class C, int R> constexpr int kWavesPerEu = C::DL > 128 || R * sizeof(typename C::Buf) > 512 ? 1 : 2;
 
 template <class C, int R, bool SPLIT>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWavesPerEu<C, R>))) void attn_paged_kernel(Args a) {
   typedef typename C::T T;
   constexpr int ROWS = Shape<C, R, SPLIT>::kRows, VL = C::VL, DL = C::DL;
   constexpr int TILES = 2 * C::SUB, KEYS = 16 * TILES;  // of a step
-  constexpr int PER = 64 / TILES;                       // steps whose pages are looked up at once
+  constexpr int PER = 64 / TILES;  // steps whose pages are looked up at once
   constexpr int LROW = DL + 4;
   __shared__ __attribute__((aligned(16))) float lds_o[SPLIT ? kWaves * 16 * R * LROW : 4];
   __shared__ float lds_m[SPLIT ? kWaves * 16 * R : 1], lds_l[SPLIT ? kWaves * 16 * R : 1];
@@ -706,36 +792,23 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves
   const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-  // tokens that no sequence holds: zeros
-  if (a.cu) {
-    const int first = min(max(a.cu[0], 0), a.total), last = min(max(a.cu[a.seqs], first), a.total);
-    for (int64_t i = blockIdx.x; i < first + a.total - last; i += gridDim.x) {
-      T* row = static_cast<T*>(a.o) + (i < first ? i : i - first + last) * (int64_t)a.heads * a.d;
-      for (int j = threadIdx.x; j < a.heads * a.d; j += kThreads) row[j] = from_f32<T>(0.f);
-    }
-  }
+  zero_others<T>(a);
   const Item it = find<ROWS>(a, x);
   if (a.split && blockIdx.x == 0 && threadIdx.x == 0) a.meta[0] = min(it.all_tiles, a.tiles);
   if (it.seq < 0) return;  // the whole block, before any barrier
   const int all_rows = it.s.n * a.group, row0 = it.tile * ROWS;
   const int rows = min(ROWS, all_rows - row0);
   const bool joined = it.splits > 1;
-  if (a.split && h == 0 && it.chunk == 0 && threadIdx.x == 0 && it.tiles_base + it.tile < a.tiles) {
-    int* m = a.meta + 1 + 4 * (int64_t)(it.tiles_base + it.tile);
-    m[0] = x;
-    m[1] = it.splits;
-    m[2] = it.s.start * a.group + row0;  // the tile's first row among all rows of a kv head
-    m[3] = rows;
-  }
+  note(a, it, x, h, row0, rows);
 
   // this wave's rows: limit[r], the keys row n of sub-tile r sees; rows past the end repeat the last
   const int w0 = row0 + (SPLIT ? 0 : wave * 16 * R);
   const int in_front = it.s.len - it.s.n;  // keys in front of the new tokens
   const auto limit_of = [&](int row) {
-    return a.causal ? max(0, in_front + min(row, all_rows - 1) / a.group + 1) : it.s.len;
+    return a.causal ? max(0, in_front + token_of(a, min(row, all_rows - 1)) + 1) : it.s.len;
   };
   C cache;
-  cache.init(a);
+  cache.init(a, h);
   typename C::Query q[R];
   int limit[R];
   const int k0 = (int)min((int64_t)it.chunk * it.keys, (int64_t)it.s.len);
@@ -746,8 +819,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves
   for (int r = 0; r < R; ++r) {
     const int row = w0 + 16 * r + n;
     const bool live = row < all_rows;
-    const int token = it.s.start + (live ? row / a.group : 0), head = h * a.group + (live ? row % a.group : 0);
-    C::query(a, static_cast<const T*>(a.q) + token * a.qt + head * a.qh, live, q[r]);
+    const int token = live ? token_of(a, row) : 0, head = h * a.group + (live ? row - token * a.group : 0);
+    C::query(a, static_cast<const T*>(a.q) + (it.s.start + token) * a.qt + head * a.qh, live, q[r]);
     limit[r] = min(limit_of(row), k1);
   }
 
@@ -767,44 +840,25 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves
   const int steps = k1 > k0 ? (k1 - k0 + KEYS - 1) / KEYS : 0;
   const int own = SPLIT ? (steps - wave + kWaves - 1) / kWaves : (w0 < all_rows ? steps : 0);
   const auto step_of = [&](int i) { return SPLIT ? wave + kWaves * i : i; };
-  int pages = -1, offs = 0;  // lane: tile (lane % TILES) of step (lane / TILES) of the batch looked up
-  const auto look_up = [&](int first) {
+  const auto look = [&](int first) {
     const int64_t key = (int64_t)k0 + (int64_t)step_of(first + lane / TILES) * KEYS + 16 * (lane % TILES);
-    pages = -1;
-    offs = 0;
-    if (key < k1) {
-      const int tile = (int)(key >> 4), slot = tile / a.tiles_per_page;
-      const int p = a.table[it.seq * a.table_stride + slot];
-      pages = p >= 0 && p < a.pages ? p : -1;
-      offs = (tile - slot * a.tiles_per_page) * 16;
-    }
-  };
-  const auto tiles_of = [&](int i, Tile (&t)[TILES]) {
-    const int at = (i % PER) * TILES;
-    const int key = k0 + step_of(i) * KEYS;
-#pragma unroll
-    for (int u = 0; u < TILES; ++u) {
-      t[u].page = __builtin_amdgcn_readlane(pages, at + u);
-      t[u].off = __builtin_amdgcn_readlane(offs, at + u);
-      t[u].rows = k1 - key - 16 * u;
-    }
+    return look_up<C::kMx>(a, it.seq, key, k1);
   };
 
   // One set of registers for a step's keys and values: the next step's keys are asked for
   // once the scores are made of this one's, its values once the products are.
   typename C::Buf b;
-  Tile t[TILES], ahead_t[TILES];
+  Look lk;
   if (own > 0) {
-    look_up(0);
-    tiles_of(0, t);
-    cache.load_k(a, h, t, b);
-    cache.load_v(a, h, t, b);
+    lk = look(0);
+    cache.load_k(lk, 0, b);
+    cache.load_v(lk, 0, b);
   }
+  constexpr uint64_t kAll = (1ull << TILES) - 1;
   for (int i = 0; i < own; ++i) {
     const int key0 = k0 + step_of(i) * KEYS;
-    bool whole = key0 + KEYS <= low;
-#pragma unroll
-    for (int u = 0; u < TILES; ++u) whole = whole && t[u].page >= 0;
+    const unsigned there = (unsigned)((lk.there >> (i % PER * TILES)) & kAll);
+    const bool whole = key0 + KEYS <= low && ((lk.whole >> (i % PER * TILES)) & kAll) == kAll;
     f32x4 s[R][TILES];
     float top[R];
 #pragma unroll
@@ -813,9 +867,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves
       for (int u = 0; u < TILES; ++u) s[r][u] = C::score(b, u, q[r]) * a.c;
     const bool more = i + 1 < own;
     if (more) {
-      if ((i + 1) % PER == 0) look_up(i + 1);
-      tiles_of(i + 1, ahead_t);
-      cache.load_k(a, h, ahead_t, b);
+      if ((i + 1) % PER == 0) lk = look(i + 1);
+      cache.load_k(lk, (i + 1) % PER * TILES, b);
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -824,7 +877,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves
         for (int u = 0; u < TILES; ++u)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const bool in = t[u].page >= 0 && key0 + 16 * u + 4 * g + j < limit[r];
+            const bool in = ((there >> u) & 1) != 0 && key0 + 16 * u + 4 * g + j < limit[r];
             s[r][u][j] = in ? s[r][u][j] : -INFINITY;
             seen[r] = seen[r] || in;
           }
@@ -869,7 +922,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves
           }
         C::prob(s[r][2 * u], s[r][2 * u + 1], p[u][r]);
       }
-    if (!whole) C::trim(b, t);
+    if (!whole) C::trim(b, k1 - key0);
 #pragma unroll
     for (int u = 0; u < C::SUB; ++u) {
       // Where some rows see a key that others do not, an Inf or a NaN among the values
@@ -879,11 +932,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves
       else
         C::template pv<R>(b, u, p[u], acc);
     }
-    if (more) {
-      cache.load_v(a, h, ahead_t, b);
-#pragma unroll
-      for (int u = 0; u < TILES; ++u) t[u] = ahead_t[u];
-    }
+    if (more) cache.load_v(lk, (i + 1) % PER * TILES, b);
   }
 
   // the rows' sums over the four lanes that share each
@@ -939,8 +988,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves
         }
       } else {
         const int full = row0 + row;
-        T* to = static_cast<T*>(a.o) +
-                ((int64_t)(it.s.start + full / a.group) * a.heads + h * a.group + full % a.group) * a.d + d;
+        T* to = row_of<T>(a, it.s.start, h, full) + d;
         const float inv = 1.f / den;
 #pragma unroll
         for (int c = 0; c < 4; ++c) to[c] = from_f32<T>(top == -INFINITY ? 0.f : sum[c] * inv);
@@ -952,8 +1000,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves
       const int row = w0 + 16 * r + n - row0;  // in the block's tile
       if (row >= rows) continue;
       const int full = row0 + row;
-      T* to = static_cast<T*>(a.o) +
-              ((int64_t)(it.s.start + full / a.group) * a.heads + h * a.group + full % a.group) * a.d;
+      T* to = row_of<T>(a, it.s.start, h, full);
       const float inv = 1.f / l[r];
       if (joined && g == 0) {
         a.ml[(place + row) * 2] = m[r];
@@ -1013,7 +1060,7 @@ template <typename T> __global__ __launch_bounds__(256) void attn_paged_join(Arg
       den += dens[i * quads + q];
     }
     const int full = row0 + row;
-    T* to = static_cast<T*>(a.o) + ((int64_t)(full / a.group) * a.heads + h * a.group + full % a.group) * a.d + 4 * q;
+    T* to = row_of<T>(a, 0, h, full) + 4 * q;
     const float inv = 1.f / den;
 #pragma unroll
     for (int c = 0; c < 4; ++c) to[c] = from_f32<T>(top == -INFINITY ? 0.f : sum[c] * inv);
@@ -1030,8 +1077,7 @@ struct Plan {
   int64_t tiles;      // row tiles at most
   int64_t items;      // blocks a kv head at most
   bool split;
-  int min_chunk;
-  int64_t target;
+  int min_chunk, target;
   int part_rows;
   int64_t part_bytes, ml_bytes, meta_bytes;
 };
@@ -1041,12 +1087,12 @@ inline Plan plan_of(int64_t seqs, int64_t total, bool packed, int64_t kv_heads, 
   Plan p{};
   const int64_t rows = total * group;
   p.wide = packed && rows > 32 * seqs;
-  p.rows = p.wide ? (rows32 && head_dim > 128 ? 64 : 128) : 16;  // kWideR
+  p.rows = p.wide ? (rows32 && head_dim > 128 ? 64 : 128) : 16;
   p.tiles = packed ? rows / p.rows + seqs : seqs * ((group + p.rows - 1) / p.rows);
   if (p.tiles < 1) p.tiles = 1;
   p.min_chunk = 512;
   const int64_t blocks = 2 * (int64_t)cu_count();
-  p.target = (blocks + kv_heads - 1) / kv_heads;
+  p.target = (int)((blocks + kv_heads - 1) / kv_heads);
   p.split = capacity > p.min_chunk && (!p.wide || p.tiles * kv_heads < blocks);
   p.items = p.tiles + (p.split ? p.target : 0);
   p.part_rows = packed ? p.rows : (int)(group < p.rows ? group : p.rows);
@@ -1058,27 +1104,36 @@ inline Plan plan_of(int64_t seqs, int64_t total, bool packed, int64_t kv_heads, 
   return p;
 }
 
+inline int log2_of(int64_t n) {  // -1: not a power of two
+  for (int i = 0; i < 31; ++i)
+    if (n == (int64_t)1 << i) return i;
+  return -1;
+}
+
 inline int check_plan(const char* who, const Plan& p, int64_t kv_heads) {
   if (p.items * kv_heads > INT32_MAX || (p.split && p.tiles * kv_heads * p.part_rows > INT32_MAX))
     return fail(PK_ERR_UNSUPPORTED, "%s: grid too large", who);
   return PK_OK;
 }
 
-template <class C> int launch(Args a, const Plan& p, hipStream_t s, const char* who) {
+inline void set_plan(Args& a, const Plan& p) {
   a.rows = p.part_rows;
   a.items = (int)p.items;
   a.tiles = (int)p.tiles;
   a.split = p.split;
   a.min_chunk = p.min_chunk;
-  a.target = p.target;
-  const dim3 grid((unsigned)(p.items * a.kv_heads));
-  if (p.wide)
-    hipLaunchKernelGGL((attn_paged_kernel<C, C::kWideR, false>), grid, dim3(kThreads), 0, s, a);
-  else
-    hipLaunchKernelGGL((attn_paged_kernel<C, 1, true>), grid, dim3(kThreads), 0, s, a);
+  a.per_chunk = 1.0 / p.target;
+}
+
+template <typename T> void launch_join(const Args& a, const Plan& p, hipStream_t s) {
   if (p.split)
-    hipLaunchKernelGGL(attn_paged_join<typename C::T>, dim3((unsigned)(p.tiles * a.kv_heads * p.part_rows)), dim3(256), 0,
-                       s, a);
+    hipLaunchKernelGGL(attn_paged_join<T>, dim3((unsigned)(p.tiles * a.kv_heads * p.part_rows)), dim3(256), 0, s, a);
+}
+
+template <class C, int R, bool SPLIT> int launch(Args a, const Plan& p, hipStream_t s, const char* who) {
+  set_plan(a, p);
+  hipLaunchKernelGGL((attn_paged_kernel<C, R, SPLIT>), dim3((unsigned)(p.items * a.kv_heads)), dim3(kThreads), 0, s, a);
+  launch_join<typename C::T>(a, p, s);
   return launched(who);
 }
 
@@ -1125,12 +1180,16 @@ inline int paged_args(const char* who, Args& a, const int64_t* strides, int64_t 
       return fail(PK_ERR_INVALID, "%s: stride %d = %lld is not a non-negative multiple of 16 bytes", who, i,
                   (long long)strides[i]);
   const int64_t row = mxfp4 ? head_dim / 2 : head_dim * e;
-  for (int i = 4; i < 8; i += 3)
-    if (strides[i] * held * 16 + row > INT32_MAX)
-      return fail(PK_ERR_UNSUPPORTED, "%s: 16 rows of a page span more than 2 GiB", who);
+  if (strides[4] * held * 16 + row > INT32_MAX)
+    return fail(PK_ERR_UNSUPPORTED, "%s: 16 rows of a page span more than 2 GiB", who);
+  for (int i = 2; i < 5; ++i)
+    if (counts[i] > 1 && strides[i] != strides[i + 3])
+      return fail(PK_ERR_UNSUPPORTED, "%s: the key and the value cache have different strides", who);
   a.qt = strides[0], a.qh = strides[1];
-  a.kp = strides[2] * held, a.kh = strides[3] * held, a.kt = (int)(strides[4] * held);
-  a.vp = strides[5] * held, a.vh = strides[6] * held, a.vt = (int)(strides[7] * held);
+  a.page = strides[2] * held, a.head = strides[3] * held, a.token = (int)(strides[4] * held);
+  a.elem = e;
+  a.tpp_shift = log2_of(page_size / 16);
+  a.group_shift = log2_of(q_heads / kv_heads);
   a.table_stride = table_stride;
   a.width = (int)table_width;
   a.pages = (int)num_pages;

@@ -1,19 +1,33 @@
 // Attention over a paged cache of q's type (attn_paged.h): the entry point and the
 // workspace query of both caches.
 #include "attn_paged.h"
+#include "attn_paged_wide.h"
 
 namespace pk {
 namespace {
 
-template <typename T> int launch_rows(const paged::Args& a, const paged::Plan& p, hipStream_t s, const char* who) {
+using namespace paged;
+
+// fp32: both shapes on the kernel of few rows, 32 (16 at 256 dims) to a wave where they are many
+template <int DL> int launch_rows32(const Args& a, const Plan& p, hipStream_t s, const char* who) {
+  constexpr int R = DL <= 128 ? 2 : 1;
+  return p.wide ? launch<Rows32<DL>, R, false>(a, p, s, who) : launch<Rows32<DL>, 1, true>(a, p, s, who);
+}
+
+template <typename T, int DL> int launch_rows16(const Args& a, const Plan& p, hipStream_t s, const char* who) {
+  return p.wide ? launch_wide<T, T, DL, 1, 1, StageRows<T, DL>>(a, p, s, who)
+                : launch<Rows16<T, DL>, 1, true>(a, p, s, who);
+}
+
+template <typename T> int launch_rows(const Args& a, const Plan& p, hipStream_t s, const char* who) {
   if constexpr (sizeof(T) == 4)
-    return a.d <= 64    ? paged::launch<paged::Rows32<64>>(a, p, s, who)
-           : a.d <= 128 ? paged::launch<paged::Rows32<128>>(a, p, s, who)
-                        : paged::launch<paged::Rows32<256>>(a, p, s, who);
+    return a.d <= 64    ? launch_rows32<64>(a, p, s, who)
+           : a.d <= 128 ? launch_rows32<128>(a, p, s, who)
+                        : launch_rows32<256>(a, p, s, who);
   else
-    return a.d <= 64    ? paged::launch<paged::Rows16<T, 64>>(a, p, s, who)
-           : a.d <= 128 ? paged::launch<paged::Rows16<T, 128>>(a, p, s, who)
-                        : paged::launch<paged::Rows16<T, 256>>(a, p, s, who);
+    return a.d <= 64    ? launch_rows16<T, 64>(a, p, s, who)
+           : a.d <= 128 ? launch_rows16<T, 128>(a, p, s, who)
+                        : launch_rows16<T, 256>(a, p, s, who);
 }
 
 }  // namespace

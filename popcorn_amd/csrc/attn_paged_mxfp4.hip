@@ -1,13 +1,22 @@
 // Attention over a paged cache held as MXFP4 (attn_paged.h).
 #include "attn_paged.h"
+#include "attn_paged_wide.h"
 
 namespace pk {
 namespace {
 
-template <typename T> int launch_mx(const paged::Args& a, const paged::Plan& p, hipStream_t s, const char* who) {
-  return a.d <= 64    ? paged::launch<paged::RowsMx<T, 64>>(a, p, s, who)
-         : a.d <= 128 ? paged::launch<paged::RowsMx<T, 128>>(a, p, s, who)
-                      : paged::launch<paged::RowsMx<T, 256>>(a, p, s, who);
+using namespace paged;
+
+template <typename T, int DL> int launch_dims(const Args& a, const Plan& p, hipStream_t s, const char* who) {
+  constexpr int TERMS = sizeof(T) == 4 ? 3 : (__is_same(T, bf16) ? 1 : 2);
+  return p.wide ? launch_wide<T, bf16, DL, TERMS, TERMS, StageMx<DL>>(a, p, s, who)
+                : launch<RowsMx<T, DL>, 1, true>(a, p, s, who);
+}
+
+template <typename T> int launch_mx(const Args& a, const Plan& p, hipStream_t s, const char* who) {
+  return a.d <= 64    ? launch_dims<T, 64>(a, p, s, who)
+         : a.d <= 128 ? launch_dims<T, 128>(a, p, s, who)
+                      : launch_dims<T, 256>(a, p, s, who);
 }
 
 }  // namespace
@@ -40,10 +49,12 @@ int pk_attn_paged_mxfp4(const void* q, const void* k_codes, const void* k_scales
       return fail(PK_ERR_INVALID, "%s: stride %d = %lld is not a non-negative multiple of 4", who, i, (long long)strides[i]);
   if (((reinterpret_cast<uintptr_t>(k_scales) | reinterpret_cast<uintptr_t>(v_scales)) & 3u) != 0)
     return fail(PK_ERR_INVALID, "%s: the scales must be 4-byte aligned", who);
-  if (head_dim > 32 && (strides[10] * 8 > INT32_MAX || strides[13] * 8 > INT32_MAX))
+  for (int i = 8; i < 11; ++i)
+    if (counts[i - 8] > 1 && strides[i] != strides[i + 3])
+      return fail(PK_ERR_UNSUPPORTED, "%s: the keys' and the values' scales have different strides", who);
+  if (head_dim > 32 && strides[10] * 8 > INT32_MAX)
     return fail(PK_ERR_UNSUPPORTED, "%s: the scales of a row span more than 2 GiB", who);
-  a.ksp = strides[8], a.ksh = strides[9], a.ksb = head_dim > 32 ? (int)strides[10] : 0;
-  a.vsp = strides[11], a.vsh = strides[12], a.vsb = head_dim > 32 ? (int)strides[13] : 0;
+  a.spage = strides[8], a.shead = strides[9], a.sblock = head_dim > 32 ? (int)strides[10] : 0;
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
     case PK_F32: return launch_mx<float>(a, p, s, who);
