@@ -75,7 +75,8 @@ struct Args {
   int tpp_shift, group_shift;  // log2 of tiles_per_page and group, or -1
   int seqs, total, heads, kv_heads, group, d;
   int causal;
-  float c;  // scale * log2(e)
+  float c;        // |scale| * log2(e), at least 1e-30
+  uint32_t flip;  // 0x80008000 where the scale is negative, for pairs of 16-bit q
   int split;       // whether sequences may be split
   int min_chunk;   // keys
   double per_chunk;  // 1 / the chunks a kv head is to have
@@ -360,7 +361,7 @@ template <typename T_, int DL_> struct Rows16 {
 #pragma unroll
     for (int j = 0; j < QN; ++j) {
       q[j] = w4{0, 0, 0, 0};
-      if (live && 32 * j + 8 * g < a.d) q[j] = *reinterpret_cast<const w4*>(row + 32 * j + 8 * g);
+      if (live && 32 * j + 8 * g < a.d) q[j] = *reinterpret_cast<const w4*>(row + 32 * j + 8 * g) ^ a.flip;
     }
   }
   __device__ __forceinline__ void load_k(const Look& l, int at, Buf& b) const {
@@ -481,6 +482,7 @@ template <int DL_> struct Rows32 {
     for (int j = 0; j < QN; ++j) {
       q[j] = f32x4{0.f, 0.f, 0.f, 0.f};
       if (live && 16 * j + 4 * g < a.d) q[j] = *reinterpret_cast<const f32x4*>(row + 16 * j + 4 * g);
+      if (a.flip) q[j] = -q[j];
     }
   }
   __device__ __forceinline__ void load_k(const Look& l, int at, Buf& b) const {
@@ -613,7 +615,7 @@ template <typename T_, int DL_> struct RowsMx {
       if (live && c < a.d) raw = ld_lane<T, 8>(row + c);
       float x[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = to_f32(raw.v[i]);
+      for (int i = 0; i < 8; ++i) x[i] = a.flip ? -to_f32(raw.v[i]) : to_f32(raw.v[i]);
       terms_of<bf16, TERMS>(x, q[j]);
     }
   }
@@ -746,6 +748,12 @@ template <typename T_, int DL_> struct RowsMx {
   }
 };
 
+// Four consecutive outputs, each rounded once
+template <typename T> __device__ __forceinline__ void store4(T* to, const f32x4& v) {
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>(to) = v;
+  else *reinterpret_cast<w2*>(to) = w2{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
+}
+
 // Zeros for the tokens that no sequence holds.
 template <typename T> __device__ __forceinline__ void zero_others(const Args& a) {
   if (!a.cu) return;
@@ -855,6 +863,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves
     cache.load_v(lk, 0, b);
   }
   constexpr uint64_t kAll = (1ull << TILES) - 1;
+  bool left = false;
   for (int i = 0; i < own; ++i) {
     const int key0 = k0 + step_of(i) * KEYS;
     const unsigned there = (unsigned)((lk.there >> (i % PER * TILES)) & kAll);
@@ -864,7 +873,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int u = 0; u < TILES; ++u) s[r][u] = C::score(b, u, q[r]) * a.c;
+      for (int u = 0; u < TILES; ++u) s[r][u] = C::score(b, u, q[r]);
     const bool more = i + 1 < own;
     if (more) {
       if ((i + 1) % PER == 0) lk = look(i + 1);
@@ -879,7 +888,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves
           for (int j = 0; j < 4; ++j) {
             const bool in = ((there >> u) & 1) != 0 && key0 + 16 * u + 4 * g + j < limit[r];
             s[r][u][j] = in ? s[r][u][j] : -INFINITY;
-            seen[r] = seen[r] || in;
+            seen[r] |= in;
           }
       } else {
         seen[r] = true;
@@ -892,13 +901,13 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves
     }
     bool over = false;
 #pragma unroll
-    for (int r = 0; r < R; ++r) over = over || top[r] > m[r] + kLag;
+    for (int r = 0; r < R; ++r) over = over || top[r] * a.c > m[r] + kLag;
     if (__any(over)) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         float t1 = fmaxf(top[r], __shfl_xor(top[r], 16, 64));
         t1 = fmaxf(t1, __shfl_xor(t1, 32, 64));
-        const float now = fmaxf(m[r], t1);
+        const float now = fmaxf(m[r], t1 * a.c);
         const float f = now == m[r] ? 1.f : __builtin_amdgcn_exp2f(m[r] - now);
         m[r] = now;
         l[r] *= f;
@@ -916,7 +925,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves
         for (int v = 0; v < 2; ++v)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float e = __builtin_amdgcn_exp2f(s[r][2 * u + v][j] - base);
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][2 * u + v][j], a.c, -base));
             s[r][2 * u + v][j] = e;
             l[r] += e;
           }
@@ -925,15 +934,46 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves
     if (!whole) C::trim(b, k1 - key0);
 #pragma unroll
     for (int u = 0; u < C::SUB; ++u) {
-      // Where some rows see a key that others do not, an Inf or a NaN among the values
-      // must stay out of the others (0 times it is a NaN): one key at a time then.
-      if (!whole && key0 + 32 * u + 32 > low && __any(C::wild(b, u)))
-        C::template pv_apart<R>(b, u, p[u], acc, [&](int r, int key) { return key0 + 32 * u + key < limit[r]; });
-      else
-        C::template pv<R>(b, u, p[u], acc);
+      // Where some rows see a key that others do not, an Inf or a NaN among the values must
+      // stay out of the others (0 times it is a NaN): such steps are left for the loop below.
+      if (!whole && key0 + KEYS > low && __any(C::wild(b, u))) left = true;
+      else C::template pv<R>(b, u, p[u], acc);
     }
     if (more) cache.load_v(lk, (i + 1) % PER * TILES, b);
   }
+
+  // The values left: one key at a time, added to the rows that see it. (Apart from the loop
+  // above, whose registers this took when it was part of it.)
+  if (left)
+    for (int i = 0; i < own; ++i) {
+      const int key0 = k0 + step_of(i) * KEYS;
+      if (key0 + KEYS <= low) continue;
+      lk = look(i);
+      cache.load_k(lk, 0, b);
+      cache.load_v(lk, 0, b);
+      C::trim(b, k1 - key0);
+#pragma unroll
+      for (int u = 0; u < C::SUB; ++u) {
+        if (!__any(C::wild(b, u))) continue;
+        typename C::Prob p[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float base = m[r] == -INFINITY ? 0.f : m[r];
+          f32x4 s[2];
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {
+            s[v] = C::score(b, 2 * u + v, q[r]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const bool in = ((lk.there >> (2 * u + v)) & 1) && key0 + 32 * u + 16 * v + 4 * g + j < limit[r];
+              s[v][j] = in ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[v][j], a.c, -base)) : 0.f;
+            }
+          }
+          C::prob(s[0], s[1], p[r]);
+        }
+        C::template pv_apart<R>(b, u, p, acc, [&](int r, int key) { return key0 + 32 * u + key < limit[r]; });
+      }
+    }
 
   // the rows' sums over the four lanes that share each
 #pragma unroll
@@ -989,9 +1029,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves
       } else {
         const int full = row0 + row;
         T* to = row_of<T>(a, it.s.start, h, full) + d;
-        const float inv = 1.f / den;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) to[c] = from_f32<T>(top == -INFINITY ? 0.f : sum[c] * inv);
+        store4(to, sum * (top == -INFINITY ? 0.f : 1.f / den));
       }
     }
   } else {
@@ -1001,7 +1039,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves
       if (row >= rows) continue;
       const int full = row0 + row;
       T* to = row_of<T>(a, it.s.start, h, full);
-      const float inv = 1.f / l[r];
+      const float inv = m[r] == -INFINITY ? 0.f : 1.f / l[r];
       if (joined && g == 0) {
         a.ml[(place + row) * 2] = m[r];
         a.ml[(place + row) * 2 + 1] = l[r];
@@ -1013,12 +1051,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves
           const int d = VL * (4 * g + c) + e;
           if (d >= a.d) continue;
           const f32x4 v = {acc[r][e][c], acc[r][e + 1][c], acc[r][e + 2][c], acc[r][e + 3][c]};
-          if (joined) {
-            *reinterpret_cast<f32x4*>(a.part + (place + row) * a.d + d) = v;
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) to[d + i] = from_f32<T>(m[r] == -INFINITY ? 0.f : v[i] * inv);
-          }
+          if (joined) *reinterpret_cast<f32x4*>(a.part + (place + row) * a.d + d) = v;
+          else store4(to + d, v * inv);
         }
     }
   }
@@ -1061,9 +1095,7 @@ template <typename T> __global__ __launch_bounds__(256) void attn_paged_join(Arg
     }
     const int full = row0 + row;
     T* to = row_of<T>(a, 0, h, full) + 4 * q;
-    const float inv = 1.f / den;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) to[c] = from_f32<T>(top == -INFINITY ? 0.f : sum[c] * inv);
+    store4(to, sum * (top == -INFINITY ? 0.f : 1.f / den));
   }
 }
 
@@ -1201,7 +1233,8 @@ inline int paged_args(const char* who, Args& a, const int64_t* strides, int64_t 
   a.group = (int)(q_heads / kv_heads);
   a.d = (int)head_dim;
   a.causal = causal;
-  a.c = softmax_scale * 1.4426950408889634f;
+  a.c = fmaxf(fabsf(softmax_scale) * 1.4426950408889634f, 1e-30f);
+  a.flip = softmax_scale < 0.f ? 0x80008000u : 0u;
   p = plan_of(seqs, total, a.cu != nullptr, kv_heads, a.group, head_dim, table_width * page_size,
               !mxfp4 && dtype == PK_F32);
   const int status = check_plan(who, p, kv_heads);

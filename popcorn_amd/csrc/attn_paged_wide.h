@@ -13,6 +13,10 @@
 // takes the same chunk of 16 consecutive rows, which the swizzle spreads over the 16
 // slots of a 256-byte bank window; V is read by transposing reads (attn_fwd.hip).
 //
+// Step t turns S(t) into P(t), then runs O += V(t)^T P(t)^T and S(t + 1) = K(t + 1) Q^T as
+// one sequence of products whose LDS fragments are read kRing products ahead; K(t + 2) and
+// V(t + 1) are asked for at its start and there at its end, at one barrier a step.
+//
 // q and P enter as TERMS values of E (attn_paged.h): one where E is q's own type.
 #pragma once
 
@@ -56,20 +60,20 @@ template <typename E, int DL> struct StageRows {
       voff[p] = vc < a.d ? row * a.token + vc * 2 : kPad;
     }
   }
-  // The tile whose halves are lanes at and at + 1 of l, into LDS, asynchronously.
-  __device__ __forceinline__ void fetch(const Look& l, int at, E* k, E* v) const {
+  __device__ __forceinline__ void fetch(const char* base, const int (&offs)[PARTS], const Look& l, int at, E* to) const {
 #pragma unroll
     for (int i = 0; i < OWN; ++i) {
       const int id = wave + kWaves * i, half = id / NI, part = id % NI;  // half is the wave's own
-      const uint64_t off = lane64(l.at, at + half);
-      const int bytes = __builtin_amdgcn_readlane(l.bytes, at + half);
-      const int to = (half * 16 * CH + part * 64) * 8;
-      attn::ld_lds16_asm(attn::make_rsrc_words(kb + off, bytes), k + to, koff[i % PARTS], 0);
-      attn::ld_lds16_asm(attn::make_rsrc_words(vb + off, bytes), v + to, voff[i % PARTS], 0);
+      const auto r = attn::make_rsrc_words(base + lane64(l.at, at + half), __builtin_amdgcn_readlane(l.bytes, at + half));
+      attn::ld_lds16_asm(r, to + (half * 16 * CH + part * 64) * 8, offs[i % PARTS], 0);
     }
   }
+  // The tile whose halves are lanes at and at + 1 of l, into LDS, asynchronously.
+  __device__ __forceinline__ void fetch_k(const Look& l, int at, E* k) const { fetch(kb, koff, l, at, k); }
+  __device__ __forceinline__ void fetch_v(const Look& l, int at, E* v) const { fetch(vb, voff, l, at, v); }
   // after the step: what was fetched lies in LDS
-  __device__ __forceinline__ void store(int, E*, E*) const { attn::lds_loads_landed(); }
+  __device__ __forceinline__ void store_k(int, E*) const { attn::lds_loads_landed(); }
+  __device__ __forceinline__ void store_v(int, E*) const {}
 };
 
 // Staging of MXFP4 rows: a thread takes eight codes and their scale into registers, and
@@ -99,38 +103,47 @@ template <int DL> struct StageMx {
       soff[i] = 8 * c < a.d ? (c / 4) * a.sblock + r : kPad;
     }
   }
-  __device__ __forceinline__ void fetch(const Look& l, int at, E*, E*) {
+  __device__ __forceinline__ void fetch(const char* rows, const char* scales, const Look& l, int at, uint32_t (&c)[OWN],
+                                        uint32_t (&e)[OWN]) const {
 #pragma unroll
     for (int i = 0; i < OWN; ++i) {
       const int half = __builtin_amdgcn_readfirstlane(row(i) / 16);  // 64 consecutive chunks lie in one half
-      const uint64_t o = lane64(l.at, at + half), so = lane64(l.scales, at + half);
       const int bytes = __builtin_amdgcn_readlane(l.bytes, at + half);
-      const int sb = bytes > 0 ? scale_bytes : 0;
-      kc[i] = __builtin_amdgcn_raw_buffer_load_b32(rsrc_of(kb + o, bytes), off[i], 0, 0);
-      ke[i] = __builtin_amdgcn_raw_buffer_load_b8(rsrc_of(ksb + so, sb), soff[i], 0, 0);
-      vc[i] = __builtin_amdgcn_raw_buffer_load_b32(rsrc_of(vb + o, bytes), off[i], 0, 0);
-      ve[i] = __builtin_amdgcn_raw_buffer_load_b8(rsrc_of(vsb + so, sb), soff[i], 0, 0);
+      c[i] = __builtin_amdgcn_raw_buffer_load_b32(rsrc_of(rows + lane64(l.at, at + half), bytes), off[i], 0, 0);
+      e[i] = __builtin_amdgcn_raw_buffer_load_b8(rsrc_of(scales + lane64(l.scales, at + half), bytes > 0 ? scale_bytes : 0),
+                                                 soff[i], 0, 0);
     }
   }
+  __device__ __forceinline__ void fetch_k(const Look& l, int at, E*) { fetch(kb, ksb, l, at, kc, ke); }
+  __device__ __forceinline__ void fetch_v(const Look& l, int at, E*) { fetch(vb, vsb, l, at, vc, ve); }
   // rows: visible keys of the tile; the scales behind them may be anything
-  __device__ __forceinline__ void store(int rows, E* k, E* v) const {
+  template <typename S>
+  __device__ __forceinline__ void store(int rows, E* to, const uint32_t (&codes)[OWN], const uint32_t (&e)[OWN], const S& swz) const {
 #pragma unroll
     for (int i = 0; i < OWN; ++i) {
-      const int r = row(i), c = chunk(i);
-      const bool in = r < rows;
-      *reinterpret_cast<uint4*>(k + (r * CH + (c ^ k_swz<DL>(r))) * 8) = mx::decode8_bf16(kc[i], mx::scale_of(in ? ke[i] : 0u));
-      *reinterpret_cast<uint4*>(v + (r * CH + (c ^ v_swz<DL>(r))) * 8) = mx::decode8_bf16(vc[i], mx::scale_of(in ? ve[i] : 0u));
+      const int r = row(i);
+      *reinterpret_cast<uint4*>(to + (r * CH + (chunk(i) ^ swz(r))) * 8) =
+          mx::decode8_bf16(codes[i], mx::scale_of(r < rows ? e[i] : 0u));
     }
+  }
+  __device__ __forceinline__ void store_k(int rows, E* k) const {
+    store(rows, k, kc, ke, [](int r) { return k_swz<DL>(r); });
+  }
+  __device__ __forceinline__ void store_v(int rows, E* v) const {
+    store(rows, v, vc, ve, [](int r) { return v_swz<DL>(r); });
   }
 };
 
+// LDS fragments in flight ahead of the product that uses them
+template <int DL> constexpr int kRing = DL > 128 ? 3 : 6;
+
 // TERMS_Q, TERMS_P: values of E that q and P are the sums of.
 template <typename T, typename E, int DL, int TERMS_Q, int TERMS_P, class Stage>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DL > 128 || TERMS_Q > 2 ? 1 : 2))) void attn_paged_wide_kernel(
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DL > 128 || TERMS_Q > 2 ? 1 : (TERMS_Q == 1 ? 3 : 2)))) void attn_paged_wide_kernel(
     Args a) {
   typedef typename attn::Mma<E>::frag Frag;
   constexpr int ROWS = 32 * kWaves, CH = DL / 8, KK = DL / 16, DT = DL / 32;
-  constexpr int PER = 32;  // steps whose pages are looked up at once: two halves each
+  constexpr int PER = 32;  // tiles whose pages are looked up at once: two halves each
   __shared__ __attribute__((aligned(16))) Shared<E, DL> lds;
   const int h = (int)(blockIdx.x % (unsigned)a.kv_heads), x = (int)(blockIdx.x / (unsigned)a.kv_heads);
   const int lane = threadIdx.x & 63, r32 = lane & 31, g = lane >> 5;
@@ -153,7 +166,6 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DL > 1
   const int chunk_end = (int)min((int64_t)k0 + it.keys, (int64_t)it.s.len);
   const int k1 = min(chunk_end, limit_of(row0 + ROWS - 1));  // keys the block goes over
   const int low = min(limit_of(w0), chunk_end);              // keys every row of the wave sees
-  const int high = w0 < all_rows ? min(limit_of(w0 + 31), k1) : 0;  // keys any of them sees
   const int limit = min(limit_of(w0 + r32), k1);
 
   Frag q[KK][TERMS_Q];
@@ -168,7 +180,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DL > 1
       if constexpr (sizeof(T) == 2 && TERMS_Q == 1) {
         w4 raw = {0, 0, 0, 0};
         if (live && c < a.d) raw = *reinterpret_cast<const w4*>(qr + c);
-        q[kk][0] = __builtin_bit_cast(Frag, raw);
+        q[kk][0] = __builtin_bit_cast(Frag, raw ^ a.flip);
       } else {
         Lane<T, 8> raw;
 #pragma unroll
@@ -176,7 +188,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DL > 1
         if (live && c < a.d) raw = ld_lane<T, 8>(qr + c);
         float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_f32(raw.v[i]);
+        for (int i = 0; i < 8; ++i) v[i] = a.flip ? -to_f32(raw.v[i]) : to_f32(raw.v[i]);
         w4 t[TERMS_Q];
         terms_of<E, TERMS_Q>(v, t);
 #pragma unroll
@@ -200,138 +212,197 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DL > 1
   const auto look = [&](int first) {
     return look_up<Stage::kMx>(a, it.seq, (int64_t)k0 + (int64_t)first * kTile + 16 * lane, k1);
   };
-  // this lane's places in a tile: a K fragment's row, and V^T's transposing reads (key
-  // rows kr + 16 c + 8 h, dims 32 dt + 16 ((lane >> 4) & 1) + 4 (lane & 3) .. + 3)
-  const int k_row = r32 * CH, k_x = k_swz<DL>(r32);
+  // this lane's places in a tile: K fragment kk (keys r32, dims 16 kk + 8 g .. + 7) at
+  // k_at ^ 16 kk, and V^T's transposing reads (key rows kr + 16 c + 8 h, dims 32 dt +
+  // 16 ((lane >> 4) & 1) + 4 (lane & 3) .. + 3)
+  const int k_at = (r32 * CH + (g ^ k_swz<DL>(r32))) * 8;
   int v_dt[DT];
   {
     const int kr = 4 * g + ((lane & 15) >> 2), vq = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), vs = v_swz<DL>(kr) / 4;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) v_dt[dt] = kr * DL + (4 * (dt ^ vs) + vq) * 8 + 4 * (lane & 1);
   }
+  const auto kfrag = [&](const E* kb, int kk) -> Frag { return *reinterpret_cast<const Frag*>(kb + (k_at ^ (16 * kk))); };
   const auto vfrag = [&](const E* vb, int c, int dt) -> Frag {
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((attn::lds_s4*)(vb + v_dt[dt] + 16 * c * DL));
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((attn::lds_s4*)(vb + v_dt[dt] + (16 * c + 8) * DL));
     return __builtin_bit_cast(Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   };
+  const auto scores = [&](const E* kb) {
+    f32x16 s;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      const Frag f = kfrag(kb, kk);
+#pragma unroll
+      for (int n = 0; n < TERMS_Q; ++n) s = attn::Mma<E>::run(f, q[kk][n], s);
+    }
+    return s;
+  };
+
+  // Where some rows see a key that others do not, an Inf or a NaN among the values must
+  // stay out of the others (0 times it is a NaN).
+  const auto wild_tile = [&](const E* vb) {
+    bool wild = false;
+#pragma unroll
+    for (int i = 0; i < DL / 16; ++i) {
+      const w4 w = *reinterpret_cast<const w4*>(vb + (i * 64 + lane) * 8);
+#pragma unroll
+      for (int n = 0; n < 4; ++n) wild |= wild2<E>(w[n]);
+    }
+    return wild;
+  };
+  bool left = false;
 
   Look lk;
+  int first = 0;  // the tile of lane 0 of lk
+  f32x16 s;
   if (steps > 0) {
     lk = look(0);
-    stage.fetch(lk, 0, lds.k[0], lds.v[0]);
-    stage.store(k1 - k0, lds.k[0], lds.v[0]);
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    stage.fetch_k(lk, 0, lds.k[0]);
+    stage.fetch_v(lk, 0, lds.v[0]);
+    stage.store_k(k1 - k0, lds.k[0]);
+    stage.store_v(k1 - k0, lds.v[0]);
+    stage.fetch_k(lk, 2, lds.k[1]);
+    stage.store_k(k1 - k0 - kTile, lds.k[1]);
+    __syncthreads();
+    s = scores(lds.k[0]);
+    __syncthreads();  // K(0) is read; the first step overwrites it
   }
-  __syncthreads();
   for (int t = 0; t < steps; ++t) {
-    const int key0 = k0 + t * kTile, at = 2 * (t % PER);
-    const unsigned there = (unsigned)(lk.there >> at) & 3u;
-    const bool whole = key0 + kTile <= low && ((lk.whole >> at) & 3u) == 3u;
-    const E *ks = lds.k[t & 1], *vs = lds.v[t & 1];
-    const bool more = t + 1 < steps;
-    if (more) {
-      if ((t + 1) % PER == 0) {
-        lk = look(t + 1);
-        __builtin_amdgcn_s_waitcnt(0x0F70);
-      }
-      stage.fetch(lk, 2 * ((t + 1) % PER), lds.k[(t + 1) & 1], lds.v[(t + 1) & 1]);
+    const int key0 = k0 + t * kTile;
+    if (t + 2 - first == PER) {
+      lk = look(t);
+      first = t;
+      __builtin_amdgcn_s_waitcnt(0x0F70);
     }
-    if (key0 < high) {
-      f32x16 s;
+    const int at = 2 * (t - first);
+    // behind the last tile these read nothing
+    stage.fetch_k(lk, at + 4, lds.k[t & 1]);
+    stage.fetch_v(lk, at + 2, lds.v[(t + 1) & 1]);
+    const bool whole = key0 + kTile <= low && ((lk.whole >> at) & 3u) == 3u;
+    const E *ks = lds.k[(t + 1) & 1], *vs = lds.v[t & 1];
+    bool wild = false;
+    if (!whole) {
+      const unsigned there = (unsigned)(lk.there >> at) & 3u;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = 0.f;
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        const Frag f = *reinterpret_cast<const Frag*>(ks + (k_row + ((2 * kk + g) ^ k_x)) * 8);
-#pragma unroll
-        for (int n = 0; n < TERMS_Q; ++n) s = attn::Mma<E>::run(f, q[kk][n], s);
+      for (int r = 0; r < 16; ++r) {
+        const bool in = (there & (1u << (r / 8))) && key0 + 8 * (r / 4) + 4 * g + r % 4 < limit;
+        s[r] = in ? s[r] : -INFINITY;
+        seen |= in;
       }
+      if (key0 + kTile > low) wild = wild_tile(vs);
+    } else {
+      seen = true;
+    }
+    float top = s[0];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] *= a.c;
-      if (!whole) {
+    for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+    if (__any(top * a.c > m + kLag)) {
+      const float now = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)) * a.c);
+      const float f = now == m ? 1.f : __builtin_amdgcn_exp2f(m - now);
+      m = now;
+      l *= f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) acc[dt] *= f;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+    Frag p[2][TERMS_P];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float e[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * c + j], a.c, -base));
+        l += e[j];
+      }
+      w4 w[TERMS_P];
+      terms_of<E, TERMS_P>(e, w);
+#pragma unroll
+      for (int n = 0; n < TERMS_P; ++n) p[c][n] = __builtin_bit_cast(Frag, w[n]);
+    }
+    if (__any(wild)) {  // its values are left for the loop below
+      left = true;
+      s = scores(ks);
+    } else {
+      constexpr int N = 2 * KK, RING = kRing<DL> < N ? kRing<DL> : N;  // 2 DT = KK products of V^T P^T, KK of S^T
+      const auto fetch = [&](int i) -> Frag { return i < KK ? vfrag(vs, i / DT, i % DT) : kfrag(ks, i - KK); };
+      Frag ring[RING];
+#pragma unroll
+      for (int i = 0; i < RING; ++i) ring[i] = fetch(i);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const Frag f = ring[i % RING];
+        if (i + RING < N) ring[i % RING] = fetch(i + RING);
+        if (i < KK) {
+#pragma unroll
+          for (int n = 0; n < TERMS_P; ++n) acc[i % DT] = attn::Mma<E>::run(f, p[i / DT][n], acc[i % DT]);
+        } else {
+          if (i == KK) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = 0.f;
+          }
+#pragma unroll
+          for (int n = 0; n < TERMS_Q; ++n) s = attn::Mma<E>::run(f, q[i - KK][n], s);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    stage.store_k(k1 - key0 - 2 * kTile, lds.k[t & 1]);
+    stage.store_v(k1 - key0 - kTile, lds.v[(t + 1) & 1]);
+    __syncthreads();
+  }
+
+  // The tiles left: their values one key at a time, added to the rows that see it. (Apart
+  // from the loop above, whose registers this took when it was part of it.)
+  if (__syncthreads_or(left)) {
+    const float base = m == -INFINITY ? 0.f : m;
+    for (int t = max(0, (min(limit_of(row0), k1) - k0) / kTile); t < steps; ++t) {
+      const int key0 = k0 + t * kTile;
+      lk = look(t);
+      __builtin_amdgcn_s_waitcnt(0x0F70);
+      stage.fetch_k(lk, 0, lds.k[0]);
+      stage.fetch_v(lk, 0, lds.v[0]);
+      stage.store_k(k1 - key0, lds.k[0]);
+      stage.store_v(k1 - key0, lds.v[0]);
+      __syncthreads();
+      if (key0 + kTile > low && __any(wild_tile(lds.v[0]))) {
+        s = scores(lds.k[0]);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const bool in = ((there >> (r / 8)) & 1) != 0 && key0 + 8 * (r / 4) + 4 * g + r % 4 < limit;
-          s[r] = in ? s[r] : -INFINITY;
-          seen = seen || in;
+          const bool in = ((lk.there >> (r / 8)) & 1) && key0 + 8 * (r / 4) + 4 * g + r % 4 < limit;
+          s[r] = in ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -base)) : 0.f;
         }
-      } else {
-        seen = true;
-      }
-      float top = s[0];
-#pragma unroll
-      for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
-      if (__any(top > m + kLag)) {
-        const float now = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
-        const float f = now == m ? 1.f : __builtin_amdgcn_exp2f(m - now);
-        m = now;
-        l *= f;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) acc[dt] *= f;
-      }
-      const float base = m == -INFINITY ? 0.f : m;
-      Frag p[2][TERMS_P];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float e[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          e[j] = __builtin_amdgcn_exp2f(s[8 * c + j] - base);
-          l += e[j];
-        }
-        w4 w[TERMS_P];
-        terms_of<E, TERMS_P>(e, w);
-#pragma unroll
-        for (int n = 0; n < TERMS_P; ++n) p[c][n] = __builtin_bit_cast(Frag, w[n]);
-      }
-      // Where some rows see a key that others do not, an Inf or a NaN among the values must
-      // stay out of the others (0 times it is a NaN): one key at a time then.
-      bool wild = false;
-      if (!whole && key0 + kTile > low) {
-#pragma unroll
-        for (int i = 0; i < DL / 16; ++i) {
-          const w4 w = *reinterpret_cast<const w4*>(vs + (i * 64 + lane) * 8);
-#pragma unroll
-          for (int n = 0; n < 4; ++n) wild = wild || wild2<E>(w[n]);
-        }
-      }
-      if (__any(wild)) {
 #pragma unroll 1
         for (int key = 0; key < kTile; ++key) {
           // key 16 c + 8 (j / 4) + 4 g + j % 4 is element j of lane half g in product c
           const int c = key >> 4, j = 4 * ((key >> 3) & 1) + (key & 3);
-          const uint32_t half = g == ((key >> 2) & 1) ? ((j & 1) ? 0xffff0000u : 0xffffu) : 0u;
-          w4 mask;
+          const bool mine = g == ((key >> 2) & 1);
+          float e[8];
 #pragma unroll
-          for (int w = 0; w < 4; ++w) mask[w] = w == j / 2 ? half : 0u;
+          for (int i = 0; i < 8; ++i) e[i] = mine && i == j ? (c ? s[8 + i] : s[i]) : 0.f;
+          w4 w[TERMS_P], mask;
+          terms_of<E, TERMS_P>(e, w);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mask[i] = mine && i == j / 2 ? ((j & 1) ? 0xffff0000u : 0xffffu) : 0u;
           const bool in = key0 + key < limit;
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) {
-            const Frag f = __builtin_bit_cast(Frag, __builtin_bit_cast(w4, vfrag(vs, c, dt)) & mask);
+            const Frag f = __builtin_bit_cast(Frag, __builtin_bit_cast(w4, vfrag(lds.v[0], c, dt)) & mask);
             f32x16 add;
 #pragma unroll
             for (int r = 0; r < 16; ++r) add[r] = 0.f;
 #pragma unroll
-            for (int n = 0; n < TERMS_P; ++n) {
-              const w4 both = c ? __builtin_bit_cast(w4, p[1][n]) : __builtin_bit_cast(w4, p[0][n]);
-              add = attn::Mma<E>::run(f, __builtin_bit_cast(Frag, both & mask), add);
-            }
+            for (int n = 0; n < TERMS_P; ++n) add = attn::Mma<E>::run(f, __builtin_bit_cast(Frag, w[n]), add);
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[dt][r] += in ? add[r] : 0.f;
           }
         }
-      } else {
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
-            const Frag f = vfrag(vs, c, dt);
-#pragma unroll
-            for (int n = 0; n < TERMS_P; ++n) acc[dt] = attn::Mma<E>::run(f, p[c][n], acc[dt]);
-          }
       }
+      __syncthreads();
     }
-    if (more) stage.store(k1 - key0 - kTile, lds.k[(t + 1) & 1], lds.v[(t + 1) & 1]);
-    __syncthreads();
   }
 
   l += __shfl_xor(l, 32, 64);
@@ -342,23 +413,20 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DL > 1
   if (row >= rows) return;
   const int64_t place = (((int64_t)x * a.kv_heads + h) * a.rows + row) * a.d;
   T* to = row_of<T>(a, it.s.start, h, row0 + row);
-  const float inv = 1.f / l;
   if (joined && g == 0) {
     a.ml[place / a.d * 2] = m;
     a.ml[place / a.d * 2 + 1] = l;
   }
+  const float inv = m == -INFINITY ? 0.f : 1.f / l;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
       const int d = 32 * dt + 8 * b + 4 * g;
-      if (d >= a.d) continue;
       const f32x4 v = {acc[dt][4 * b], acc[dt][4 * b + 1], acc[dt][4 * b + 2], acc[dt][4 * b + 3]};
-      if (joined) {
-        *reinterpret_cast<f32x4*>(a.part + place + d) = v;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) to[d + i] = from_f32<T>(m == -INFINITY ? 0.f : v[i] * inv);
+      if (d < a.d) {
+        if (joined) *reinterpret_cast<f32x4*>(a.part + place + d) = v;
+        else store4(to + d, v * inv);
       }
     }
 }
