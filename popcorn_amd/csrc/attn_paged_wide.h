@@ -139,7 +139,7 @@ template <int DL> constexpr int kRing = DL > 128 ? 3 : 6;
 
 // TERMS_Q, TERMS_P: values of E that q and P are the sums of.
 template <typename T, typename E, int DL, int TERMS_Q, int TERMS_P, class Stage>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DL > 128 || TERMS_Q > 2 ? 1 : (TERMS_Q == 1 ? 3 : 2)))) void attn_paged_wide_kernel(
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DL > 128 || TERMS_Q > 2 ? 1 : 2))) void attn_paged_wide_kernel(
     Args a) {
   typedef typename attn::Mma<E>::frag Frag;
   constexpr int ROWS = 32 * kWaves, CH = DL / 8, KK = DL / 16, DT = DL / 32;
@@ -213,28 +213,40 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DL > 1
     return look_up<Stage::kMx>(a, it.seq, (int64_t)k0 + (int64_t)first * kTile + 16 * lane, k1);
   };
   // this lane's places in a tile: K fragment kk (keys r32, dims 16 kk + 8 g .. + 7) at
-  // k_at ^ 16 kk, and V^T's transposing reads (key rows kr + 16 c + 8 h, dims 32 dt +
-  // 16 ((lane >> 4) & 1) + 4 (lane & 3) .. + 3)
+  // k_at ^ 16 kk, and V^T's transposing reads (key rows v_kr + 16 c + 8 h, dims 32 dt +
+  // 16 ((lane >> 4) & 1) + 4 (lane & 3) .. + 3) at v_at ^ 32 dt
   const int k_at = (r32 * CH + (g ^ k_swz<DL>(r32))) * 8;
-  int v_dt[DT];
-  {
-    const int kr = 4 * g + ((lane & 15) >> 2), vq = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), vs = v_swz<DL>(kr) / 4;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) v_dt[dt] = kr * DL + (4 * (dt ^ vs) + vq) * 8 + 4 * (lane & 1);
-  }
-  const auto kfrag = [&](const E* kb, int kk) -> Frag { return *reinterpret_cast<const Frag*>(kb + (k_at ^ (16 * kk))); };
-  const auto vfrag = [&](const E* vb, int c, int dt) -> Frag {
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((attn::lds_s4*)(vb + v_dt[dt] + 16 * c * DL));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((attn::lds_s4*)(vb + v_dt[dt] + (16 * c + 8) * DL));
+  const int v_kr = 4 * g + ((lane & 15) >> 2);
+  const int v_at = v_kr * DL + (v_swz<DL>(v_kr) + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) * 8 + 4 * (lane & 1);
+  // (from k_at and v_at in the step's buffers, which the compiler is kept from splitting into
+  // an address for each kk and dt: registers that the loop does not have)
+  const auto kfrag = [&](int k_now, int kk) -> Frag {
+    return *reinterpret_cast<const Frag*>(&lds.k[0][0] + (k_now ^ (16 * kk)));
+  };
+  const auto k_in = [&](int buf) {
+    int k_now = k_at + buf * (kTile * DL);
+    asm volatile("" : "+v"(k_now));
+    return k_now;
+  };
+  const auto v_in = [&](int buf) {
+    int v_now = v_at + buf * (kTile * DL);
+    asm volatile("" : "+v"(v_now));
+    return v_now;
+  };
+  const auto vfrag = [&](int v_now, int c, int dt) -> Frag {
+    const E* at = &lds.v[0][0] + (v_now ^ (32 * dt));
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((attn::lds_s4*)(at + 16 * c * DL));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((attn::lds_s4*)(at + (16 * c + 8) * DL));
     return __builtin_bit_cast(Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   };
-  const auto scores = [&](const E* kb) {
+  const auto scores = [&](int buf) {
+    const int k_now = k_in(buf);
     f32x16 s;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
-      const Frag f = kfrag(kb, kk);
+      const Frag f = kfrag(k_now, kk);
 #pragma unroll
       for (int n = 0; n < TERMS_Q; ++n) s = attn::Mma<E>::run(f, q[kk][n], s);
     }
@@ -245,7 +257,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DL > 1
   // stay out of the others (0 times it is a NaN).
   const auto wild_tile = [&](const E* vb) {
     bool wild = false;
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < DL / 16; ++i) {
       const w4 w = *reinterpret_cast<const w4*>(vb + (i * 64 + lane) * 8);
 #pragma unroll
@@ -268,7 +280,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DL > 1
     stage.fetch_k(lk, 2, lds.k[1]);
     stage.store_k(k1 - k0 - kTile, lds.k[1]);
     __syncthreads();
-    s = scores(lds.k[0]);
+    s = scores(0);
     __syncthreads();  // K(0) is read; the first step overwrites it
   }
   for (int t = 0; t < steps; ++t) {
@@ -283,7 +295,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DL > 1
     stage.fetch_k(lk, at + 4, lds.k[t & 1]);
     stage.fetch_v(lk, at + 2, lds.v[(t + 1) & 1]);
     const bool whole = key0 + kTile <= low && ((lk.whole >> at) & 3u) == 3u;
-    const E *ks = lds.k[(t + 1) & 1], *vs = lds.v[t & 1];
+    const E* vs = lds.v[t & 1];
     bool wild = false;
     if (!whole) {
       const unsigned there = (unsigned)(lk.there >> at) & 3u;
@@ -325,10 +337,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DL > 1
     }
     if (__any(wild)) {  // its values are left for the loop below
       left = true;
-      s = scores(ks);
+      s = scores((t + 1) & 1);
     } else {
       constexpr int N = 2 * KK, RING = kRing<DL> < N ? kRing<DL> : N;  // 2 DT = KK products of V^T P^T, KK of S^T
-      const auto fetch = [&](int i) -> Frag { return i < KK ? vfrag(vs, i / DT, i % DT) : kfrag(ks, i - KK); };
+      const int k_now = k_in((t + 1) & 1), v_now = v_in(t & 1);
+      const auto fetch = [&](int i) -> Frag { return i < KK ? vfrag(v_now, i / DT, i % DT) : kfrag(k_now, i - KK); };
       Frag ring[RING];
 #pragma unroll
       for (int i = 0; i < RING; ++i) ring[i] = fetch(i);
@@ -369,7 +382,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DL > 1
       stage.store_v(k1 - key0, lds.v[0]);
       __syncthreads();
       if (key0 + kTile > low && __any(wild_tile(lds.v[0]))) {
-        s = scores(lds.k[0]);
+        s = scores(0);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const bool in = ((lk.there >> (r / 8)) & 1) && key0 + 8 * (r / 4) + 4 * g + r % 4 < limit;
@@ -390,7 +403,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DL > 1
           const bool in = key0 + key < limit;
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) {
-            const Frag f = __builtin_bit_cast(Frag, __builtin_bit_cast(w4, vfrag(lds.v[0], c, dt)) & mask);
+            const Frag f = __builtin_bit_cast(Frag, __builtin_bit_cast(w4, vfrag(v_in(0), c, dt)) & mask);
             f32x16 add;
 #pragma unroll
             for (int r = 0; r < 16; ++r) add[r] = 0.f;
