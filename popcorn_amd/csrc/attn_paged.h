@@ -35,6 +35,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 #include "api.h"
 #include "attn_common.h"
 #include "common.h"
@@ -79,7 +81,7 @@ struct Args {
   uint32_t flip;  // 0x80008000 where the scale is negative, for pairs of 16-bit q
   int split;       // whether sequences may be split
   int min_chunk;   // keys
-  double per_chunk;  // 1 / the chunks a kv head is to have
+  float target, at_once;  // blocks that run at once: a kv head's share, and all
   int items;       // blocks a kv head, and row tiles: what the workspace has room for, and offsets
   int tiles;       // that do not rise may ask for more
   // partial sums: part [items][kv_heads][rows][d], ml [items][kv_heads][rows][2], meta [1 + 4 * row tiles]
@@ -89,9 +91,19 @@ struct Args {
   int rows;  // rows of a block's tile that partial sums have room for
 };
 
-__device__ __forceinline__ int64_t wave_sum64(int64_t v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+// Inclusive sums over a wave's lanes: within rows of 16 lanes, then rows onto the rows behind.
+template <typename V> __device__ __forceinline__ V scan(V v) {
+  const auto moved = [](V x, auto ctrl, auto rows) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value,
+                                                             decltype(rows)::value, 0xF, false));
+  };
+  typedef std::integral_constant<int, 0xF> All;
+  v += moved(v, std::integral_constant<int, 0x111>(), All());  // the lane 1, 2, 4 and 8 in front, in the row
+  v += moved(v, std::integral_constant<int, 0x112>(), All());
+  v += moved(v, std::integral_constant<int, 0x114>(), All());
+  v += moved(v, std::integral_constant<int, 0x118>(), All());
+  v += moved(v, std::integral_constant<int, 0x142>(), std::integral_constant<int, 0xA>());  // last lane of rows 0, 2 onto 1, 3
+  v += moved(v, std::integral_constant<int, 0x143>(), std::integral_constant<int, 0xC>());  // lane 31 onto rows 2 and 3
   return v;
 }
 
@@ -127,6 +139,28 @@ struct Item {
   int all_tiles;
 };
 
+// Keys of a chunk, from the sum of row tiles times keys: an even share of the blocks that
+// run at once where that cuts the sequences into no more blocks than those, else a third of
+// it, so that blocks of different lengths fill each other's gaps. 48 sequences of 1000 to
+// 32768 keys in 4 bits, 8 heads: 159 us at an even share, 142 at half, 137 at a third, 153 at
+// a sixth; two of 131071 keys: 189, 198, 201 at the first three.
+constexpr int kParts = 3;
+
+template <int ROWS> __device__ __forceinline__ int chunk_of(const Args& a, float work) {
+  // 1.02: a fp32 sum of up to 2^18 terms a lane is off by less, and the room for partial sums counts on it
+  const float even = fminf(work * 1.02f / a.target, 1e9f);
+  const int keys = max(((int)even + 64) / 64 * 64, a.min_chunk);
+  const float per = 1.f / (float)keys;
+  float blocks = 0.f;
+  for (int i = threadIdx.x & 63; i < a.seqs; i += 64) {
+    const Seq s = seq_of(a, i);
+    blocks += (float)(((unsigned)s.n * (unsigned)a.group + ROWS - 1) / ROWS) * fmaxf(ceilf((float)s.len * per), 1.f);
+  }
+  blocks = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scan(blocks)), 63));
+  return __builtin_amdgcn_readfirstlane(
+      blocks * a.kv_heads <= a.at_once ? keys : max(((int)(even / kParts) + 64) / 64 * 64, a.min_chunk));
+}
+
 // Which piece of work block x is, the same in every lane; seq < 0: none. Each wave
 // finds it alone, 64 sequences at a time: the lane of a sequence counts its blocks.
 template <int ROWS> __device__ __forceinline__ Item find(const Args& a, int x) {
@@ -137,20 +171,16 @@ template <int ROWS> __device__ __forceinline__ Item find(const Args& a, int x) {
   int tiles = 0;
   Seq s = {0, 0, 0};
   if (a.split) {
-    int64_t work = 0;
+    float work = 0.f;
     for (int i = lane; i < a.seqs; i += 64) {
       s = seq_of(a, i);
       const int rt = (int)(((unsigned)s.n * (unsigned)a.group + ROWS - 1) / ROWS);
-      work += (int64_t)rt * s.len;
+      work += (float)rt * (float)s.len;
       tiles += rt;
     }
-    work = wave_sum64(work);
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) tiles += __shfl_xor(tiles, off, 64);
-    tiles = __builtin_amdgcn_readfirstlane(tiles);
-    // one more than the quotient: never fewer keys than an even share
-    const int even = (int)fmin((double)work * a.per_chunk, 1073741000.0) + 1;
-    it.keys = __builtin_amdgcn_readfirstlane(max((even + 63) / 64 * 64, a.min_chunk));
+    work = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scan(work)), 63));
+    tiles = __builtin_amdgcn_readlane(scan(tiles), 63);
+    it.keys = chunk_of<ROWS>(a, work);
   }
   it.all_tiles = tiles;
   int before = 0, tiles_before = 0;
@@ -163,12 +193,7 @@ template <int ROWS> __device__ __forceinline__ Item find(const Args& a, int x) {
     const int rt = (int)(((unsigned)s.n * (unsigned)a.group + ROWS - 1) / ROWS);
     const int splits = a.split ? max(1, (int)(((unsigned)s.len + (unsigned)it.keys - 1) / (unsigned)it.keys)) : 1;
     const int mine = rt * splits;
-    int upto = mine, rts = rt;  // inclusive sums over the lanes
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int p = __shfl_up(upto, off, 64), q = __shfl_up(rts, off, 64);
-      if (lane >= off) upto += p, rts += q;
-    }
+    const int upto = scan(mine), rts = scan(rt);
     const int rel = x - before;
     const uint64_t found = __ballot(rel >= upto - mine && rel < upto);
     if (found != 0) {
@@ -559,23 +584,24 @@ template <int DL_> struct Rows32 {
   }
 };
 
-// Rows of MXFP4 codes, 64 keys a step. A lane's K piece is DL / 4 consecutive
+// Rows of MXFP4 codes, 64 or 128 keys a step. A lane's K piece is DL / 4 consecutive
 // channels (16 bytes are one block of 32), a V piece VL, inside one block. They become
 // bf16, exactly, in registers; q and P are as many bf16 terms as their type has bits
 // for (bf16 one, fp16 two, fp32 three), and P of bf16 two as well, so nothing is rounded on the way.
 template <typename T_, int DL_> struct RowsMx {
   typedef T_ T;
-  static constexpr int DL = DL_, VL = DL / 16, SUB = 2, QN = DL / 32;
   static constexpr int TERMS = sizeof(T) == 4 ? 3 : (__is_same(T, bf16) ? 1 : 2), PTERMS = sizeof(T) == 4 ? 3 : 2;
+  static constexpr int DL = DL_, VL = DL / 16, QN = DL / 32;
+  static constexpr int SUB = DL <= 128 && TERMS == 1 ? 4 : 2, NT = 2 * SUB;
   static constexpr bool kMx = true;
   static constexpr int KW = DL >= 128 ? 4 : 2;     // words of codes in a K piece
   static constexpr int KP = DL >= 128 ? DL / 128 : 1;  // K pieces of a row in a lane
   static constexpr int VW = VL >= 8 ? VL / 8 : 1;  // words of codes of a V row in a lane (half a word at DL 64)
   struct Buf {
-    uint32_t k[4][KP][KW];
-    uint32_t ke[4][KP];  // scale bytes
-    uint32_t v[16][VW];
-    uint32_t ve[4];  // scale bytes of the lane's four keys of each tile
+    uint32_t k[NT][KP][KW];
+    uint32_t ke[NT][KP];  // scale bytes
+    uint32_t v[4 * NT][VW];
+    uint32_t ve[NT];  // scale bytes of the lane's four keys of each tile
   };
   typedef w4 Query[QN][TERMS];
   typedef w4 Prob[PTERMS];
@@ -621,7 +647,7 @@ template <typename T_, int DL_> struct RowsMx {
   }
   __device__ __forceinline__ void load_k(const Look& l, int at, Buf& b) const {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < NT; ++u) {
       const auto kr = paged::tile_rsrc(kb, l.at, l.bytes, at + u);
       const auto sr = rsrc_of(kse_b + lane64(l.scales, at + u), (l.there >> (at + u)) & 1 ? scale_bytes : 0);
 #pragma unroll
@@ -640,7 +666,7 @@ template <typename T_, int DL_> struct RowsMx {
   }
   __device__ __forceinline__ void load_v(const Look& l, int at, Buf& b) const {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < NT; ++u) {
       const auto vr = paged::tile_rsrc(vb, l.at, l.bytes, at + u);
       const auto sr = rsrc_of(vse_b + lane64(l.scales, at + u), (l.there >> (at + u)) & 1 ? scale_bytes : 0);
 #pragma unroll
@@ -663,7 +689,7 @@ template <typename T_, int DL_> struct RowsMx {
   static __device__ __forceinline__ void trim(Buf& b, int rows) {
     const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < NT; ++u) {
       const int n = min(max(rows - 16 * u - 4 * g, 0), 4);
       b.ve[u] &= n == 4 ? 0xffffffffu : (1u << (8 * n)) - 1u;
     }
@@ -760,7 +786,7 @@ template <typename T> __device__ __forceinline__ void zero_others(const Args& a)
   const int first = min(max(a.cu[0], 0), a.total), last = min(max(a.cu[a.seqs], first), a.total);
   for (int64_t i = blockIdx.x; i < first + a.total - last; i += gridDim.x) {
     T* row = static_cast<T*>(a.o) + (i < first ? i : i - first + last) * (int64_t)a.heads * a.d;
-    for (int j = threadIdx.x; j < a.heads * a.d; j += kThreads) row[j] = from_f32<T>(0.f);
+    for (int j = threadIdx.x; j < a.heads * a.d; j += blockDim.x) row[j] = from_f32<T>(0.f);
   }
 }
 
@@ -788,7 +814,8 @@ template <class C, int R, bool SPLIT> struct Shape {
 template <class C, int R> constexpr int kWavesPerEu = C::DL > 128 || R * sizeof(typename C::Buf) > 512 ? 1 : 2;
 
 template <class C, int R, bool SPLIT>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWavesPerEu<C, R>))) void attn_paged_kernel(Args a) {
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWavesPerEu<C, R>))) void
+attn_paged_kernel(Args a) {
   typedef typename C::T T;
   constexpr int ROWS = Shape<C, R, SPLIT>::kRows, VL = C::VL, DL = C::DL;
   constexpr int TILES = 2 * C::SUB, KEYS = 16 * TILES;  // of a step
@@ -915,9 +942,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves
         for (int e = 0; e < VL; ++e) acc[r][e] *= f;
       }
     }
-    typename C::Prob p[C::SUB][R];
+    if (!whole) C::trim(b, k1 - key0);
 #pragma unroll
-    for (int u = 0; u < C::SUB; ++u)
+    for (int u = 0; u < C::SUB; ++u) {
+      typename C::Prob p[R];
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const float base = m[r] == -INFINITY ? 0.f : m[r];
@@ -929,15 +957,12 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves
             s[r][2 * u + v][j] = e;
             l[r] += e;
           }
-        C::prob(s[r][2 * u], s[r][2 * u + 1], p[u][r]);
+        C::prob(s[r][2 * u], s[r][2 * u + 1], p[r]);
       }
-    if (!whole) C::trim(b, k1 - key0);
-#pragma unroll
-    for (int u = 0; u < C::SUB; ++u) {
       // Where some rows see a key that others do not, an Inf or a NaN among the values must
       // stay out of the others (0 times it is a NaN): such steps are left for the loop below.
       if (!whole && key0 + KEYS > low && __any(C::wild(b, u))) left = true;
-      else C::template pv<R>(b, u, p[u], acc);
+      else C::template pv<R>(b, u, p, acc);
     }
     if (more) cache.load_v(lk, (i + 1) % PER * TILES, b);
   }
@@ -1058,44 +1083,60 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves
   }
 }
 
-// Joins the chunks of split row tiles, in their order: a block takes one row, a lane
-// four dims of every kLanes-th chunk.
-template <typename T> __global__ __launch_bounds__(256) void attn_paged_join(Args a) {
-  __shared__ f32x4 sums[256];
-  __shared__ float dens[256];
-  const int row = (int)(blockIdx.x % (unsigned)a.rows);
-  const int h = (int)(blockIdx.x / (unsigned)a.rows % (unsigned)a.kv_heads);
-  const int tile = (int)(blockIdx.x / (unsigned)a.rows / (unsigned)a.kv_heads);
+// Joins the chunks of split row tiles: a block takes kJoinRows rows of a tile (one where a
+// tile has at most 16), a thread four dims of every parts-th chunk of a row, where the
+// rows leave threads for more than one part; parts are then added in their order.
+constexpr int kJoinThreads = 256;
+inline __host__ __device__ int join_rows(int rows) { return rows > 16 ? 8 : 1; }
+
+template <typename T> __global__ __launch_bounds__(kJoinThreads) void attn_paged_join(Args a) {
+  __shared__ f32x4 sums[kJoinThreads];
+  __shared__ float dens[kJoinThreads];
+  const int each = join_rows(a.rows), groups = (a.rows + each - 1) / each;
+  const int from = (int)(blockIdx.x % (unsigned)groups) * each;
+  const int h = (int)(blockIdx.x / (unsigned)groups % (unsigned)a.kv_heads);
+  const int tile = (int)(blockIdx.x / (unsigned)groups / (unsigned)a.kv_heads);
   if (tile >= a.meta[0]) return;
   const int* m = a.meta + 1 + 4 * (int64_t)tile;
   const int first = m[0], splits = m[1], row0 = m[2], rows = m[3];
-  if (splits <= 1 || row >= rows) return;  // the whole block, before any barrier
-  if (first < 0 || splits > a.items - first || row0 < 0 || row0 > a.total * a.group - rows) return;
-  const int quads = a.d / 4, lanes = 256 / quads;
-  const int q = threadIdx.x % quads, s0 = threadIdx.x / quads;
-  const auto at = [&](int s) { return ((int64_t)(first + s) * a.kv_heads + h) * a.rows + row; };
-  float top = -INFINITY;
-  for (int s = 0; s < splits; ++s) top = fmaxf(top, a.ml[at(s) * 2]);
-  const float base = top == -INFINITY ? 0.f : top;
-  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  float den = 0.f;
-  if (s0 < lanes)
-    for (int s = s0; s < splits; s += lanes) {
-      const float f = __builtin_amdgcn_exp2f(a.ml[at(s) * 2] - base);
-      sum += *reinterpret_cast<const f32x4*>(a.part + at(s) * a.d + 4 * q) * f;
-      den += a.ml[at(s) * 2 + 1] * f;
+  if (splits <= 1 || from >= rows) return;  // the whole block, before any barrier
+  if (first < 0 || splits > a.items - first || row0 < 0 || row0 > a.total * a.group - rows || rows > a.rows) return;
+  const int quads = a.d / 4, slots = kJoinThreads / quads;
+  int parts = 1;
+  while (2 * parts * each <= slots && 2 * parts <= splits) parts *= 2;
+  const int q = threadIdx.x % quads, slot = threadIdx.x / quads, part = slot % parts;
+  const int at_once = slots / parts, end = min(from + each, rows);
+  for (int base_row = from; base_row < end; base_row += at_once) {
+    const int row = base_row + slot / parts;
+    const bool mine = slot < at_once * parts && row < end;
+    float top = -INFINITY;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    float den = 0.f;
+    if (mine) {
+      const int64_t step = (int64_t)a.kv_heads * a.rows, at = ((int64_t)first * a.kv_heads + h) * a.rows + row;
+      const float* ml = a.ml + 2 * at;
+      const float* part_sum = a.part + at * a.d + 4 * q;
+#pragma unroll 8
+      for (int s = 0; s < splits; ++s) top = fmaxf(top, ml[2 * s * step]);
+      const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll 4
+      for (int s = part; s < splits; s += parts) {
+        const float f = __builtin_amdgcn_exp2f(ml[2 * s * step] - base);
+        sum += *reinterpret_cast<const f32x4*>(part_sum + s * step * a.d) * f;
+        den += ml[2 * s * step + 1] * f;
+      }
     }
-  sums[threadIdx.x] = sum;
-  dens[threadIdx.x] = den;
-  __syncthreads();
-  if (s0 == 0) {
-    for (int i = 1; i < lanes; ++i) {
-      sum += sums[i * quads + q];
-      den += dens[i * quads + q];
+    sums[threadIdx.x] = sum;
+    dens[threadIdx.x] = den;
+    __syncthreads();
+    if (mine && part == 0) {
+      for (int i = 1; i < parts; ++i) {
+        sum += sums[threadIdx.x + i * quads];
+        den += dens[threadIdx.x + i * quads];
+      }
+      store4(row_of<T>(a, 0, h, row0 + row) + 4 * q, sum * (top == -INFINITY ? 0.f : 1.f / den));
     }
-    const int full = row0 + row;
-    T* to = row_of<T>(a, 0, h, full) + 4 * q;
-    store4(to, sum * (top == -INFINITY ? 0.f : 1.f / den));
+    __syncthreads();
   }
 }
 
@@ -1109,7 +1150,7 @@ struct Plan {
   int64_t tiles;      // row tiles at most
   int64_t items;      // blocks a kv head at most
   bool split;
-  int min_chunk, target;
+  int min_chunk, target, at_once;
   int part_rows;
   int64_t part_bytes, ml_bytes, meta_bytes;
 };
@@ -1123,10 +1164,14 @@ inline Plan plan_of(int64_t seqs, int64_t total, bool packed, int64_t kv_heads, 
   p.tiles = packed ? rows / p.rows + seqs : seqs * ((group + p.rows - 1) / p.rows);
   if (p.tiles < 1) p.tiles = 1;
   p.min_chunk = 512;
-  const int64_t blocks = 2 * (int64_t)cu_count();
-  p.target = (int)((blocks + kv_heads - 1) / kv_heads);
-  p.split = capacity > p.min_chunk && (!p.wide || p.tiles * kv_heads < blocks);
-  p.items = p.tiles + (p.split ? p.target : 0);
+  p.at_once = 2 * cu_count();  // eight waves a CU, what their registers allow
+  p.target = (int)((p.at_once + kv_heads - 1) / kv_heads);
+  p.split = capacity > p.min_chunk && (!p.wide || p.tiles * kv_heads < p.at_once);
+  p.items = p.tiles;
+  if (p.split) {  // a chunk is at least a kParts-th of an even share, and min_chunk keys
+    const int64_t most = p.tiles * ((capacity + p.min_chunk - 1) / p.min_chunk);
+    p.items = most < p.tiles + kParts * p.target ? most : p.tiles + kParts * p.target;
+  }
   p.part_rows = packed ? p.rows : (int)(group < p.rows ? group : p.rows);
   if (p.split) {
     p.part_bytes = (p.items * kv_heads * p.part_rows * head_dim * 4 + 255) / 256 * 256;
@@ -1154,17 +1199,21 @@ inline void set_plan(Args& a, const Plan& p) {
   a.tiles = (int)p.tiles;
   a.split = p.split;
   a.min_chunk = p.min_chunk;
-  a.per_chunk = 1.0 / p.target;
+  a.target = (float)p.target;
+  a.at_once = (float)p.at_once;
 }
 
 template <typename T> void launch_join(const Args& a, const Plan& p, hipStream_t s) {
   if (p.split)
-    hipLaunchKernelGGL(attn_paged_join<T>, dim3((unsigned)(p.tiles * a.kv_heads * p.part_rows)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(attn_paged_join<T>,
+                       dim3((unsigned)(p.tiles * a.kv_heads * ((a.rows + join_rows(a.rows) - 1) / join_rows(a.rows)))),
+                       dim3(kJoinThreads), 0, s, a);
 }
 
 template <class C, int R, bool SPLIT> int launch(Args a, const Plan& p, hipStream_t s, const char* who) {
   set_plan(a, p);
-  hipLaunchKernelGGL((attn_paged_kernel<C, R, SPLIT>), dim3((unsigned)(p.items * a.kv_heads)), dim3(kThreads), 0, s, a);
+  hipLaunchKernelGGL((attn_paged_kernel<C, R, SPLIT>), dim3((unsigned)(p.items * a.kv_heads)),
+                     dim3(kThreads), 0, s, a);
   launch_join<typename C::T>(a, p, s);
   return launched(who);
 }
