@@ -58,7 +58,7 @@ template <typename T> struct alignas(16) Chunk {
   __device__ __forceinline__ void store(T* p) const {
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-      reinterpret_cast<u32x4_any*>(p)[i] = reinterpret_cast<const u32x4*>(v)[i];
+      __builtin_nontemporal_store(reinterpret_cast<const u32x4*>(v)[i], reinterpret_cast<u32x4_any*>(p) + i);
   }
 };
 
