@@ -1143,7 +1143,9 @@ template <typename T> __global__ __launch_bounds__(kJoinThreads) void attn_paged
 // ---------------------------------------------------------------- host side
 
 // Rows of a block's tile, chosen by the rows a sequence has on average: 16 that the
-// waves split the keys of, or 128 that they share out.
+// waves split the keys of, or 128 that they share out. (fp32 q over more than 128 dims of
+// MXFP4 stays at 16: its three terms of q and P, 256 dims wide, do not fit the registers
+// of a wave with 32 rows.)
 struct Plan {
   bool wide;
   int rows;           // of a tile
@@ -1156,11 +1158,11 @@ struct Plan {
 };
 
 inline Plan plan_of(int64_t seqs, int64_t total, bool packed, int64_t kv_heads, int64_t group, int64_t head_dim,
-                    int64_t capacity, bool rows32) {
+                    int64_t capacity, bool f32, bool mxfp4) {
   Plan p{};
   const int64_t rows = total * group;
-  p.wide = packed && rows > 32 * seqs;
-  p.rows = p.wide ? (rows32 && head_dim > 128 ? 64 : 128) : 16;
+  p.wide = packed && rows > 32 * seqs && !(f32 && mxfp4 && head_dim > 128);
+  p.rows = p.wide ? (f32 && head_dim > 128 ? 64 : 128) : 16;
   p.tiles = packed ? rows / p.rows + seqs : seqs * ((group + p.rows - 1) / p.rows);
   if (p.tiles < 1) p.tiles = 1;
   p.min_chunk = 512;
@@ -1285,7 +1287,7 @@ inline int paged_args(const char* who, Args& a, const int64_t* strides, int64_t 
   a.c = fmaxf(fabsf(softmax_scale) * 1.4426950408889634f, 1e-30f);
   a.flip = softmax_scale < 0.f ? 0x80008000u : 0u;
   p = plan_of(seqs, total, a.cu != nullptr, kv_heads, a.group, head_dim, table_width * page_size,
-              !mxfp4 && dtype == PK_F32);
+              dtype == PK_F32, mxfp4);
   const int status = check_plan(who, p, kv_heads);
   if (status != PK_OK) return status;
   const int64_t need = p.part_bytes + p.ml_bytes + p.meta_bytes;

@@ -42,7 +42,7 @@ int64_t pk_attn_paged_workspace(int64_t num_seqs, int64_t total, int packed, int
   if (total == 0 || q_heads == 0) return 0;
   if (kv_heads == 0 || q_heads % kv_heads != 0 || total * q_heads > INT32_MAX || num_seqs > (1 << 24)) return -1;
   const paged::Plan p = paged::plan_of(num_seqs, total, packed != 0, kv_heads, q_heads / kv_heads, head_dim, capacity,
-                                        !mxfp4 && dtype == PK_F32);
+                                        dtype == PK_F32, mxfp4 != 0);
   return p.part_bytes + p.ml_bytes + p.meta_bytes;
 }
 

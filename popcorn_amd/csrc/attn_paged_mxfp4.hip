@@ -9,8 +9,10 @@ using namespace paged;
 
 template <typename T, int DL> int launch_dims(const Args& a, const Plan& p, hipStream_t s, const char* who) {
   constexpr int TERMS = sizeof(T) == 4 ? 3 : (__is_same(T, bf16) ? 1 : 2);
-  return p.wide ? launch_wide<T, bf16, DL, TERMS, TERMS, StageMx<DL>>(a, p, s, who)
-                : launch<RowsMx<T, DL>, 1, true>(a, p, s, who);
+  if constexpr (TERMS < 3 || DL <= 128) {
+    if (p.wide) return launch_wide<T, bf16, DL, TERMS, TERMS, StageMx<DL>>(a, p, s, who);
+  }
+  return launch<RowsMx<T, DL>, 1, true>(a, p, s, who);
 }
 
 template <typename T> int launch_mx(const Args& a, const Plan& p, hipStream_t s, const char* who) {

@@ -33,10 +33,11 @@ constexpr int kTile = 32;
 template <int DL> __device__ __forceinline__ int k_swz(int r) { return DL == 64 ? (r >> 1) & 7 : r & 15; }
 template <int DL> __device__ __forceinline__ int v_swz(int r) { return DL == 64 ? 4 * ((r >> 1) & 1) : 4 * (r & 3); }
 
-// Tiles of E in LDS, two of each (the step's and the next one's)
+// Tiles of E in LDS, two of each (the step's and the next one's), and zeros in the place
+// of values that a step leaves out
 template <typename E, int DL> struct Shared {
   E k[2][kTile * DL];
-  E v[2][kTile * DL];
+  E v[3][kTile * DL];
 };
 
 // Staging of 16-bit rows: whole 16-byte slots, written by the load itself.
@@ -267,6 +268,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DL > 1
   };
   bool left = false;
 
+  for (int i = threadIdx.x; i < kTile * DL / 8; i += kThreads) reinterpret_cast<w4*>(lds.v[2])[i] = w4{0, 0, 0, 0};
   Look lk;
   int first = 0;  // the tile of lane 0 of lk
   f32x16 s;
@@ -335,33 +337,32 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DL > 1
 #pragma unroll
       for (int n = 0; n < TERMS_P; ++n) p[c][n] = __builtin_bit_cast(Frag, w[n]);
     }
-    if (__any(wild)) {  // its values are left for the loop below
-      left = true;
-      s = scores((t + 1) & 1);
-    } else {
-      constexpr int N = 2 * KK, RING = kRing<DL> < N ? kRing<DL> : N;  // 2 DT = KK products of V^T P^T, KK of S^T
-      const int k_now = k_in((t + 1) & 1), v_now = v_in(t & 1);
-      const auto fetch = [&](int i) -> Frag { return i < KK ? vfrag(v_now, i / DT, i % DT) : kfrag(k_now, i - KK); };
-      Frag ring[RING];
+    // the values of a wild tile are left for the loop below: zeros in their place (a branch
+    // around the products cost the loop fourteen registers)
+    const bool out = __any(wild);
+    left |= out;
+    constexpr int N = 2 * KK, RING = kRing<DL> < N ? kRing<DL> : N;  // 2 DT = KK products of V^T P^T, KK of S^T
+    const int k_now = k_in((t + 1) & 1), v_now = v_in(out ? 2 : t & 1);
+    const auto fetch = [&](int i) -> Frag { return i < KK ? vfrag(v_now, i / DT, i % DT) : kfrag(k_now, i - KK); };
+    Frag ring[RING];
 #pragma unroll
-      for (int i = 0; i < RING; ++i) ring[i] = fetch(i);
+    for (int i = 0; i < RING; ++i) ring[i] = fetch(i);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const Frag f = ring[i % RING];
-        if (i + RING < N) ring[i % RING] = fetch(i + RING);
-        if (i < KK) {
+    for (int i = 0; i < N; ++i) {
+      const Frag f = ring[i % RING];
+      if (i + RING < N) ring[i % RING] = fetch(i + RING);
+      if (i < KK) {
 #pragma unroll
-          for (int n = 0; n < TERMS_P; ++n) acc[i % DT] = attn::Mma<E>::run(f, p[i / DT][n], acc[i % DT]);
-        } else {
-          if (i == KK) {
+        for (int n = 0; n < TERMS_P; ++n) acc[i % DT] = attn::Mma<E>::run(f, p[i / DT][n], acc[i % DT]);
+      } else {
+        if (i == KK) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = 0.f;
-          }
-#pragma unroll
-          for (int n = 0; n < TERMS_Q; ++n) s = attn::Mma<E>::run(f, q[i - KK][n], s);
+          for (int r = 0; r < 16; ++r) s[r] = 0.f;
         }
-        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < TERMS_Q; ++n) s = attn::Mma<E>::run(f, q[i - KK][n], s);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
     stage.store_k(k1 - key0 - 2 * kTile, lds.k[t & 1]);
     stage.store_v(k1 - key0 - kTile, lds.v[(t + 1) & 1]);
