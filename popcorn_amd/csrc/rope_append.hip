@@ -82,7 +82,7 @@ struct Turn {
 // code: towards zero, the last bit set where something was cut off. A border
 // between codes has two significant bits, so no value reaches or crosses one.
 __device__ __forceinline__ float sticky(double y) {
-  if (!(fabs(y) < 3.4028236692093846e38)) return (float)y * INFINITY;  // 2^128 and on, Inf and NaN: not finite
+  if (!(fabs(y) <= 3.4028234663852886e38)) return (float)y * INFINITY;  // past the largest fp32, Inf and NaN: not finite
   float r = (float)y;
   if (fabs((double)r) > fabs(y)) r = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, r) - 1u);
   if ((double)r != y) r = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, r) | 1u);
