@@ -389,7 +389,7 @@ int64_t pk_attn_paged_workspace(int64_t num_seqs, int64_t total, int packed, int
  * nothing is read back, so a captured call may be replayed with other contents.
  * What the pages hold behind a sequence's keys is not looked at. strides[8] = q
  * (token, head), k_cache, v_cache (page, head, token), in elements, multiples of
- * 16 bytes like every pointer. head_dim a multiple of 8 up to 256. workspace:
+ * 16 bytes like every pointer; v_cache's are k_cache's. head_dim a multiple of 8 up to 256. workspace:
  * pk_attn_paged_workspace() bytes, 16-byte aligned.
  */
 int pk_attn_paged(const void* q, const void* k_cache, const void* v_cache, const int* block_table, const int* cache_lens,
@@ -401,7 +401,8 @@ int pk_attn_paged(const void* q, const void* k_cache, const void* v_cache, const
 /*
  * The same over an MXFP4 cache, for q of any dtype: strides[14] = q (token, head),
  * k_codes, v_codes (page, head, token, multiples of 16 bytes), k_scales, v_scales
- * (page, head, block, multiples of 4). head_dim a multiple of 32 up to 256.
+ * (page, head, block, multiples of 4), the keys' and the values' alike. head_dim a
+ * multiple of 32 up to 256.
  */
 int pk_attn_paged_mxfp4(const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
                         const void* v_scales, const int* block_table, const int* cache_lens, const int* cu_seqlens,

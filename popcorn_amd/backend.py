@@ -261,6 +261,11 @@ def _aligned(unit: int, *tensors) -> bool:
                                                 for n, s in zip(t.shape[:-1], t.stride())) for t in tensors)
 
 
+def _alike(a, b) -> bool:
+    """The same strides, where a dimension has more than one place."""
+    return all(n < 2 or s == t for n, s, t in zip(a.shape, a.stride(), b.stride()))
+
+
 def attn_paged_supported(q, k_cache, v_cache, block_table, cache_lens, cu_seqlens, causal, softmax_scale) -> bool:
     return (
         _on_hip(q, k_cache, v_cache, block_table, cache_lens, cu_seqlens)
@@ -269,6 +274,7 @@ def attn_paged_supported(q, k_cache, v_cache, block_table, cache_lens, cu_seqlen
         and _attn_head_dim(q.shape[2])
         and _cache_supported(q.shape[2], k_cache.shape[1], k_cache, v_cache)
         and k_cache.shape[3] == q.shape[2]
+        and _alike(k_cache, v_cache)
         and _aligned(16, k_cache, v_cache)
     )
 
@@ -279,6 +285,8 @@ def attn_paged_mxfp4_supported(q, k_codes, k_scales, v_codes, v_scales, block_ta
         _on_hip(q, k_codes, k_scales, v_codes, v_scales, block_table, cache_lens, cu_seqlens)
         and _table_supported(q, k_codes, block_table, cache_lens, cu_seqlens)
         and _mxfp4_supported(q.shape[2], k_codes.shape[1], (k_codes, v_codes), (k_scales, v_scales))
+        and _alike(k_codes, v_codes)
+        and _alike(k_scales, v_scales)
         and _aligned(16, k_codes, v_codes)
         and _aligned(4, k_scales, v_scales)
     )

@@ -1082,8 +1082,8 @@ def attn_paged(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor,
     cu_seqlens [sequences + 1] (int32). Sequence i has the first cache_lens[i] keys of the
     pages block_table[i] (both int32); the last of its new tokens is the last key, and when
     causal each attends the keys up to its own. k_cache, v_cache [pages, kv_heads,
-    page_size, head_dim] of q's type, page_size a multiple of 16, rows and pages a multiple
-    of 16 bytes apart; head_dim as for `attn`. A token without a key, or of no sequence,
+    page_size, head_dim] of q's type and of the same strides, page_size a multiple of 16, rows
+    and pages a multiple of 16 bytes apart; head_dim as for `attn`. A token without a key, or of no sequence,
     gets zeros; keys on a page outside the pool are left out. Nothing is read back to the
     host: a captured call may be replayed with other tables and lengths. No gradient.
     Repeated calls give the same bits; how a sequence's keys are split follows the batch.
@@ -1101,6 +1101,7 @@ def attn_paged_mxfp4(q: Tensor, k_codes: Tensor, k_scales: Tensor, v_codes: Tens
                      softmax_scale: float | None = None) -> Tensor:
     """`attn_paged` over a cache held as MXFP4 (see `rope_append_mxfp4`), for q of any of the three types.
 
+    The two codes have the same strides, and so have the two scales (multiples of 4 bytes).
     The cached values enter as they stand; q in fp16 or fp32 is not rounded to do so.
     """
     if not _compiling():

@@ -401,6 +401,72 @@ def test_append_strides_and_far_rows():
     check(got, exact(yq.cpu(), *small, near, lens, None, True, None), BF, d, 16)
 
 
+def _far(shape, gap, at, dtype, buf=None):
+    """A zeroed view of `shape` [3, heads, a, b] whose pages lie `gap` bytes apart, `at` bytes into a buffer."""
+    size = dtype.itemsize
+    n = shape[1] * shape[2] * shape[3]
+    if buf is None:
+        buf = torch.empty((2 * gap + 8 * n * size) // size, dtype=dtype, device=DEV)
+    view = buf.as_strided(shape, (gap // size, shape[2] * shape[3], shape[3], 1), at // size)
+    return view.zero_(), buf
+
+
+@pytest.mark.parametrize("news", [None, [40, 33]], ids=str)
+@pytest.mark.parametrize("mxfp4", [False, True], ids=["rows", "mxfp4"])
+def test_pages_four_gib_apart(mxfp4, news):
+    """Offsets past 32 bits, of keys, values and scales, in attention and in appending."""
+    hkv, ps, d, gap = 2, 16, 64, (1 << 32) + 4096
+    lens, table = [40, 33], torch.tensor([[2, 0, 1], [1, 2, 0]], dtype=torch.int32)
+    n = 2 if news is None else sum(news)
+    cache = cache_of(3, hkv, ps, d, BF, 5)
+    if mxfp4:
+        held = [mxfp4_of(c) for c in cache]
+        rows = [values_of(*h) for h in held]
+        flat = [t for h in held for t in h]
+    else:
+        rows = flat = list(cache)
+    views, buf = [], None
+    for t in flat:
+        view, buf = _far(tuple(t.shape), gap, sum(2 * v[0].numel() * v.element_size() for v in views), t.dtype, buf)
+        views.append(view)
+    assert len({v.stride(0) for v in views}) == 1
+    for v, t in zip(views, flat):
+        v.copy_(t)
+    q = torch.randn(n, 8, d, generator=torch.Generator().manual_seed(6)).to(BF)
+    cu = None if news is None else torch.tensor([0, news[0], n], dtype=torch.int32)
+    op = impls.attn_paged_mxfp4 if mxfp4 else impls.attn_paged
+    got = op(q.to(DEV), *views, table.to(DEV), torch.tensor(lens, dtype=torch.int32).to(DEV), None if cu is None else cu.to(DEV))
+    check(got, exact(q, *rows, table, lens, cu, True, None), BF, d, 40, mxfp4)
+    append = impls.rope_append_mxfp4 if mxfp4 else impls.rope_append
+    k, v = (torch.randn(2, hkv, d, generator=torch.Generator().manual_seed(s)).to(BF) for s in (7, 8))
+    one, none = torch.ones(1, d // 2), torch.zeros(1, d // 2)
+    args = q[:2], k, v, one, none, torch.zeros(2, dtype=torch.int64), torch.tensor([2 * ps + 3, ps + 15])
+    want = [t.clone() for t in flat]
+    (R.rope_append_mxfp4 if mxfp4 else R.rope_append)(*args, *want)
+    append(*(t.to(DEV) for t in args), *views)
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(views, want))
+
+
+def test_rotated_keys_past_the_largest_fp32_are_nan_blocks():
+    """x cos + partner sin between the largest fp32 and 2^128, in 64 bits: no fp32 value; one below it is finite."""
+    top = torch.finfo(torch.float32).max
+    k = torch.zeros(2, 1, 64)
+    k[0, 0, 3], k[0, 0, 3 + 32] = top, 2.0 ** 101  # top + 2^101, less than half a step above top
+    k[1, 0, 3], k[1, 0, 3 + 32] = top, -(2.0 ** 101)
+    cos, sin = torch.ones(1, 32), torch.full((1, 32), -1.0)
+    cos[:, :3], cos[:, 4:], sin[:, :3], sin[:, 4:] = 1, 1, 0, 0
+    args = k, k, k, cos, sin, torch.zeros(2, dtype=torch.int32), torch.arange(2, dtype=torch.int32)
+    outs = []
+    for dev, op in (("cpu", R.rope_append_mxfp4), (DEV, impls.rope_append_mxfp4)):
+        held = [torch.zeros(1, 1, 16, 32, dtype=torch.uint8), torch.zeros(1, 1, 2, 16, dtype=torch.uint8)]
+        held = [t.to(dev) for t in (*held, *(t.clone() for t in held))]
+        ys = op(*(t.to(dev) for t in args), *held)
+        outs.append([t.cpu() for t in (*ys[1:], *held)])
+    assert outs[0][0][0, 0, :32].isnan().all() and outs[0][0][1, 0, :32].isfinite().all()
+    assert all(torch.equal(a.nan_to_num(7.0) if a.is_floating_point() else a, b.nan_to_num(7.0) if b.is_floating_point() else b)
+               for a, b in zip(*outs))
+
+
 # ------------------------------------------------------------------ as a program uses them
 
 
@@ -583,3 +649,56 @@ def test_refusals():
     assert not none.any()
     yq, yk = impls.rope_append(q[:0], k[:0], k[:0], cos, cos, at[:0], at[:0], *cache)
     assert yq.shape == (0, 4, 64) and yk.shape == (0, 2, 64)
+
+
+def test_caches_of_different_strides_are_refused():
+    cache = [c.to(DEV) for c in cache_of(4, 2, 16, 64, BF, 1)]
+    held = [t.to(DEV) for c in cache_of(4, 2, 16, 64, BF, 1) for t in mxfp4_of(c)]
+    q = torch.randn(2, 4, 64, device=DEV).to(BF)
+    table, lens = torch.zeros(2, 2, dtype=torch.int32, device=DEV), torch.ones(2, dtype=torch.int32, device=DEV)
+    other = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in held]
+    with pytest.raises(_lib.KernelError, match="different strides"):
+        impls.attn_paged(q, cache[0], cache[1].transpose(1, 2).contiguous().transpose(1, 2), table, lens)
+    with pytest.raises(_lib.KernelError, match="codes|key and the value"):
+        impls.attn_paged_mxfp4(q, held[0], held[1], other[2], held[3], table, lens)
+    with pytest.raises(_lib.KernelError, match="scales have different strides"):
+        impls.attn_paged_mxfp4(q, held[0], held[1], held[2], other[3], table, lens)
+    assert torch.equal(impls.attn_paged(q, *cache, table, lens), impls.attn_paged(q, *cache, table, lens))
+
+
+def test_records_and_routes(monkeypatch, tmp_path):
+    """Through the dispatch: each op graded against its reference by the harness, and then served by the backend."""
+    from popcorn_amd import backend, compat
+    from popcorn_amd.compat import store
+
+    monkeypatch.setattr(store, "BUNDLED_REPORTS", tmp_path / "bundled")
+    backend.register(compat)
+    g = torch.Generator().manual_seed(0)
+    tokens, hq, hkv, d, ps, pages = 24, 8, 2, 64, 16, 12
+    q, k, v = (torch.randn(tokens, h, d, generator=g).to(BF).to(DEV) for h in (hq, hkv, hkv))
+    angle = torch.rand(64, d // 2, generator=g) * 6.28
+    cos, sin = angle.cos().to(BF).to(DEV), angle.sin().to(BF).to(DEV)  # one float type, as a recorded call has
+    at, slots = torch.arange(tokens, device=DEV), torch.randperm(pages * ps, generator=g)[:tokens].to(DEV)
+    cache = [c.to(DEV) for c in cache_of(pages, hkv, ps, d, BF, 1)]
+    held = [t.to(DEV) for c in cache_of(pages, hkv, ps, d, BF, 1) for t in mxfp4_of(c)]
+    table = torch.randperm(pages, generator=g).int().view(3, 4).to(DEV)
+    lens = torch.tensor([60, 33, 17], dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0, 10, 11, tokens], dtype=torch.int32, device=DEV)
+    calls = {"rope_append": (q, k, v, cos, sin, at, slots, *cache), "rope_append_mxfp4": (q, k, v, cos, sin, at, slots, *held),
+             "attn_paged": (q, *cache, table, lens, cu), "attn_paged_mxfp4": (q, *held, table, lens, cu)}
+    for name, args in calls.items():
+        op = compat.KERNELS[name]
+        op.tuner.forget()
+        with torch.no_grad():
+            [record] = op.benchmark(*args, backend=backend.BACKEND)
+            assert record.result.status == "pass", (name, record.result.status, record.result.reason)
+            assert not record.result.grad and record.result.benchmarked
+            op(*args)
+        assert op.tuner.last_choice() == backend.BACKEND, name
+        op.tuner.forget()
+    with torch.no_grad():  # single tokens and fp32 tables: no one config to record, served in registration order
+        for name, args in (("attn_paged", (q[:3], *cache, table, lens)), ("attn_paged_mxfp4", (q[:3], *held, table, lens)),
+                           ("rope_append", (q, k, v, cos.float(), sin.float(), at, slots, *cache))):
+            compat.KERNELS[name](*args)
+            assert compat.KERNELS[name].tuner.last_choice() == backend.BACKEND, name
+            compat.KERNELS[name].tuner.forget()
