@@ -18,7 +18,9 @@
 //
 // Bound by HBM: q, k and v in, yq, yk and two cache rows out. A few tokens are
 // bound by the latency of one pass of loads, so the heads split over blocks until
-// the grid has about eight blocks a CU.
+// the grid has about eight blocks a CU. 16384 bf16 tokens of 32/8 heads of 128: 98.5 us,
+// 4.5 TB/s; 8192 into MXFP4: 53 us, 4.1 TB/s; 32 tokens: 5.7 us, a launch and its loads.
+// What is written is not read again here, and its stores bypass the caches (102.5 us without).
 #include "api.h"
 #include "common.h"
 #include "mxfp4.h"
