@@ -236,21 +236,21 @@ struct Look {
   uint64_t whole, there;  // lanes whose tile has 16 visible keys, and any page
 };
 
-// key: of this lane's tile; k1: the end of the visible ones
+// key: of this lane's tile; k1: the end of the visible ones, at least 1. Every lane looks,
+// those behind the last key where it lies, and selects: in a branch that only some lanes
+// take, the compiler (ROCm 7.2) moved other values to other registers in front of its end,
+// while it still left the rest out, and theirs were lost.
 template <bool MX> __device__ __forceinline__ Look look_up(const Args& a, int seq, int64_t key, int k1) {
-  Look l = {0, 0, 0, 0, 0};
-  int rows = 0;
-  if (key < k1) {
-    const int tile = (int)(key >> 4), slot = a.tpp_shift >= 0 ? tile >> a.tpp_shift : tile / a.tiles_per_page;
-    const int p = a.table[seq * a.table_stride + slot];
-    if (p >= 0 && p < a.pages) {
-      const int row = (tile - slot * a.tiles_per_page) * 16;
-      rows = min(k1 - (int)key, 16);
-      l.at = (uint64_t)p * a.page + (uint64_t)row * (unsigned)a.token;
-      l.bytes = (rows - 1) * a.token + (MX ? a.d / 2 : a.d * (int)a.elem);
-      if constexpr (MX) l.scales = (uint64_t)p * a.spage + row;
-    }
-  }
+  Look l;
+  const int tile = (int)(min(key, (int64_t)(k1 - 1)) >> 4);
+  const int slot = a.tpp_shift >= 0 ? tile >> a.tpp_shift : tile / a.tiles_per_page;
+  const int p = a.table[seq * a.table_stride + slot];
+  const bool in = key < k1 && p >= 0 && p < a.pages;
+  const int page = in ? p : 0, row = (tile - slot * a.tiles_per_page) * 16;
+  const int rows = in ? (int)min(k1 - key, (int64_t)16) : 0;
+  l.at = (uint64_t)page * a.page + (uint64_t)row * (unsigned)a.token;
+  l.bytes = in ? (rows - 1) * a.token + (MX ? a.d / 2 : a.d * (int)a.elem) : 0;
+  l.scales = MX ? (uint64_t)page * a.spage + row : 0;
   l.whole = __ballot(rows == 16);
   l.there = __ballot(rows > 0);
   return l;
