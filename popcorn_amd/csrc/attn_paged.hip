@@ -14,9 +14,8 @@ template <int DL> int launch_rows32(const Args& a, const Plan& p, hipStream_t s,
   return p.wide ? launch<Rows32<DL>, R, false>(a, p, s, who) : launch<Rows32<DL>, 1, true>(a, p, s, who);
 }
 
-template <typename T, int DL> int launch_rows16(const Args& a, const Plan& p, hipStream_t s, const char* who) {
-  return p.wide ? launch_wide<T, T, DL, 1, 1, StageRows<T, DL>>(a, p, s, who)
-                : launch<Rows16<T, DL>, 1, true>(a, p, s, who);
+template <typename T, int DL> int launch_wide16(const Args& a, const Plan& p, hipStream_t s, const char* who) {
+  return launch_wide<T, T, DL, 1, 1, StageRows<T, DL>>(a, p, s, who);
 }
 
 template <typename T> int launch_rows(const Args& a, const Plan& p, hipStream_t s, const char* who) {
@@ -24,10 +23,16 @@ template <typename T> int launch_rows(const Args& a, const Plan& p, hipStream_t 
     return a.d <= 64    ? launch_rows32<64>(a, p, s, who)
            : a.d <= 128 ? launch_rows32<128>(a, p, s, who)
                         : launch_rows32<256>(a, p, s, who);
+  else if (p.wide)
+    return a.d <= 64    ? launch_wide16<T, 64>(a, p, s, who)
+           : a.d <= 96  ? launch_wide16<T, 96>(a, p, s, who)
+           : a.d <= 128 ? launch_wide16<T, 128>(a, p, s, who)
+           : a.d <= 192 ? launch_wide16<T, 192>(a, p, s, who)
+                        : launch_wide16<T, 256>(a, p, s, who);
   else
-    return a.d <= 64    ? launch_rows16<T, 64>(a, p, s, who)
-           : a.d <= 128 ? launch_rows16<T, 128>(a, p, s, who)
-                        : launch_rows16<T, 256>(a, p, s, who);
+    return a.d <= 64    ? launch<Rows16<T, 64>, 1, true>(a, p, s, who)
+           : a.d <= 128 ? launch<Rows16<T, 128>, 1, true>(a, p, s, who)
+                        : launch<Rows16<T, 256>, 1, true>(a, p, s, who);
 }
 
 }  // namespace

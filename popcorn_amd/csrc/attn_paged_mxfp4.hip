@@ -7,18 +7,22 @@ namespace {
 
 using namespace paged;
 
-template <typename T, int DL> int launch_dims(const Args& a, const Plan& p, hipStream_t s, const char* who) {
+template <typename T, int DL> int launch_wide_mx(const Args& a, const Plan& p, hipStream_t s, const char* who) {
   constexpr int TERMS = sizeof(T) == 4 ? 3 : (__is_same(T, bf16) ? 1 : 2);
-  if constexpr (TERMS < 3 || DL <= 128) {
-    if (p.wide) return launch_wide<T, bf16, DL, TERMS, TERMS, StageMx<DL>>(a, p, s, who);
-  }
-  return launch<RowsMx<T, DL>, 1, true>(a, p, s, who);
+  return launch_wide<T, bf16, DL, TERMS, TERMS, StageMx<DL>>(a, p, s, who);
 }
 
 template <typename T> int launch_mx(const Args& a, const Plan& p, hipStream_t s, const char* who) {
-  return a.d <= 64    ? launch_dims<T, 64>(a, p, s, who)
-         : a.d <= 128 ? launch_dims<T, 128>(a, p, s, who)
-                      : launch_dims<T, 256>(a, p, s, who);
+  if (p.wide) {
+    if constexpr (sizeof(T) == 2)  // fp32 at more than 128 dims is never wide (plan_of)
+      if (a.d > 128) return a.d <= 192 ? launch_wide_mx<T, 192>(a, p, s, who) : launch_wide_mx<T, 256>(a, p, s, who);
+    return a.d <= 64   ? launch_wide_mx<T, 64>(a, p, s, who)
+           : a.d <= 96 ? launch_wide_mx<T, 96>(a, p, s, who)
+                       : launch_wide_mx<T, 128>(a, p, s, who);
+  }
+  return a.d <= 64    ? launch<RowsMx<T, 64>, 1, true>(a, p, s, who)
+         : a.d <= 128 ? launch<RowsMx<T, 128>, 1, true>(a, p, s, who)
+                      : launch<RowsMx<T, 256>, 1, true>(a, p, s, who);
 }
 
 }  // namespace

@@ -11,7 +11,9 @@
 // block and not once a wave. Each tile is two halves of 16 keys, which lie in one page
 // each. LDS rows are unpadded, chunk c of row r at slot c ^ swz(r): a K fragment read
 // takes the same chunk of 16 consecutive rows, which the swizzle spreads over the 16
-// slots of a 256-byte bank window; V is read by transposing reads (attn_fwd.hip).
+// slots of a 256-byte bank window; V is read by transposing reads (attn_fwd.hip). Rows are
+// laid out for 64, 96, 128, 192 or 256 dims: rows of 96 and 192 already start at four and
+// two different places of the window, and swizzles of two and three bits do the rest.
 //
 // Step t turns S(t) into P(t), then runs O += V(t)^T P(t)^T and S(t + 1) = K(t + 1) Q^T as
 // one sequence of products whose LDS fragments are read kRing products ahead; K(t + 2) and
@@ -34,8 +36,18 @@ using attn::s16x4;
 
 constexpr int kTile = 32;
 
-template <int DL> __device__ __forceinline__ int k_swz(int r) { return DL == 64 ? (r >> 1) & 7 : r & 15; }
-template <int DL> __device__ __forceinline__ int v_swz(int r) { return DL == 64 ? 4 * ((r >> 1) & 1) : 4 * (r & 3); }
+template <int DL> __device__ __forceinline__ int k_swz(int r) {
+  return DL == 96 ? (r >> 2) & 3 : (DL % 128 == 64 ? (r >> 1) & 7 : r & 15);
+}
+template <int DL> __device__ __forceinline__ int v_swz(int r) {
+  return DL == 96 ? 0 : (DL % 128 == 64 ? 4 * ((r >> 1) & 1) : 4 * (r & 3));
+}
+// Element of a row that lies `dims` (a multiple of 16) behind the one at `at`: the bits that
+// a swizzle reaches, below the lowest one set in DL, are flipped, and the others added.
+template <int DL> __device__ __forceinline__ int behind(int at, int dims) {
+  constexpr int LOW = (DL & -DL) - 1;
+  return (at ^ (dims & LOW)) + (dims & ~LOW);
+}
 
 // Tiles of E in LDS, two of each (the step's and the next one's), and zeros in the place
 // of values that a step leaves out
@@ -48,8 +60,8 @@ template <typename E, int DL> struct Shared {
 template <typename E, int DL> struct StageRows {
   static constexpr bool kMx = false;
   static constexpr int CH = DL / 8, NI = 16 * CH / 64;  // chunks of a row; wave instructions of a half tile
-  static constexpr int OWN = 2 * NI / kWaves;           // of both halves, a wave's
-  static constexpr int PARTS = NI > kWaves ? NI / kWaves : 1;  // different places in a half among them
+  static constexpr int OWN = (2 * NI + kWaves - 1) / kWaves;             // of both halves, a wave's
+  static constexpr int PARTS = NI % kWaves == 0 ? NI / kWaves : OWN;  // different places in a half among them
   const char *kb, *vb;
   int wave, koff[PARTS], voff[PARTS];
 
@@ -69,6 +81,7 @@ template <typename E, int DL> struct StageRows {
 #pragma unroll
     for (int i = 0; i < OWN; ++i) {
       const int id = wave + kWaves * i, half = id / NI, part = id % NI;  // half is the wave's own
+      if (2 * NI % kWaves != 0 && id >= 2 * NI) break;
       const auto r = attn::make_rsrc_words(base + lane64(l.at, at + half), __builtin_amdgcn_readlane(l.bytes, at + half));
       attn::ld_lds16_asm(r, to + (half * 16 * CH + part * 64) * 8, offs[i % PARTS], 0);
     }
@@ -86,8 +99,7 @@ template <typename E, int DL> struct StageRows {
 template <int DL> struct StageMx {
   typedef bf16 E;
   static constexpr bool kMx = true;
-  static constexpr int CH = DL / 8, OWN = kTile * CH / kThreads;
-  static constexpr int PER_HALF = OWN > 1 ? OWN / 2 : 1;
+  static constexpr int CH = DL / 8, ALL = kTile * CH, OWN = (ALL + kThreads - 1) / kThreads;
   const char *kb, *vb, *ksb, *vsb;
   int scale_bytes;
   int off[OWN], soff[OWN];
@@ -95,6 +107,10 @@ template <int DL> struct StageMx {
 
   static __device__ __forceinline__ int row(int i) { return (i * kThreads + (int)threadIdx.x) / CH; }
   static __device__ __forceinline__ int chunk(int i) { return (i * kThreads + (int)threadIdx.x) % CH; }
+  // whether this wave has chunks i at all
+  static __device__ __forceinline__ bool has(int i) {
+    return ALL % kThreads == 0 || i * kThreads + (int)__builtin_amdgcn_readfirstlane(threadIdx.x) < ALL;
+  }
   __device__ __forceinline__ void init(const Args& a, int h, int) {
     kb = static_cast<const char*>(a.k) + h * a.head;
     vb = static_cast<const char*>(a.v) + h * a.head;
@@ -112,6 +128,7 @@ template <int DL> struct StageMx {
                                         uint32_t (&e)[OWN]) const {
 #pragma unroll
     for (int i = 0; i < OWN; ++i) {
+      if (!has(i)) break;
       const int half = __builtin_amdgcn_readfirstlane(row(i) / 16);  // 64 consecutive chunks lie in one half
       const int bytes = __builtin_amdgcn_readlane(l.bytes, at + half);
       c[i] = __builtin_amdgcn_raw_buffer_load_b32(rsrc_of(rows + lane64(l.at, at + half), bytes), off[i], 0, 0);
@@ -126,6 +143,7 @@ template <int DL> struct StageMx {
   __device__ __forceinline__ void store(int rows, E* to, const uint32_t (&codes)[OWN], const uint32_t (&e)[OWN], const S& swz) const {
 #pragma unroll
     for (int i = 0; i < OWN; ++i) {
+      if (!has(i)) break;
       const int r = row(i);
       *reinterpret_cast<uint4*>(to + (r * CH + (chunk(i) ^ swz(r))) * 8) =
           mx::decode8_bf16(codes[i], mx::scale_of(r < rows ? e[i] : 0u));
@@ -217,16 +235,16 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DL > 1
   const auto look = [&](int first) {
     return look_up<Stage::kMx>(a, it.seq, (int64_t)k0 + (int64_t)first * kTile + 16 * lane, k1);
   };
-  // this lane's places in a tile: K fragment kk (keys r32, dims 16 kk + 8 g .. + 7) at
-  // k_at ^ 16 kk, and V^T's transposing reads (key rows v_kr + 16 c + 8 h, dims 32 dt +
-  // 16 ((lane >> 4) & 1) + 4 (lane & 3) .. + 3) at v_at ^ 32 dt
+  // this lane's places in a tile: K fragment kk (keys r32, dims 16 kk + 8 g .. + 7) 16 kk
+  // behind k_at, and V^T's transposing reads (key rows v_kr + 16 c + 8 h, dims 32 dt +
+  // 16 ((lane >> 4) & 1) + 4 (lane & 3) .. + 3) 32 dt behind v_at
   const int k_at = (r32 * CH + (g ^ k_swz<DL>(r32))) * 8;
   const int v_kr = 4 * g + ((lane & 15) >> 2);
   const int v_at = v_kr * DL + (v_swz<DL>(v_kr) + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) * 8 + 4 * (lane & 1);
   // (from k_at and v_at in the step's buffers, which the compiler is kept from splitting into
   // an address for each kk and dt: registers that the loop does not have)
   const auto kfrag = [&](int k_now, int kk) -> Frag {
-    return *reinterpret_cast<const Frag*>(&lds.k[0][0] + (k_now ^ (16 * kk)));
+    return *reinterpret_cast<const Frag*>(&lds.k[0][0] + behind<DL>(k_now, 16 * kk));
   };
   const auto k_in = [&](int buf) {
     int k_now = k_at + buf * (kTile * DL);
@@ -239,7 +257,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DL > 1
     return v_now;
   };
   const auto vfrag = [&](int v_now, int c, int dt) -> Frag {
-    const E* at = &lds.v[0][0] + (v_now ^ (32 * dt));
+    const E* at = &lds.v[0][0] + behind<DL>(v_now, 32 * dt);
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((attn::lds_s4*)(at + 16 * c * DL));
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((attn::lds_s4*)(at + (16 * c + 8) * DL));
     return __builtin_bit_cast(Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
