@@ -33,8 +33,8 @@
 // other lengths.
 //
 // Bound by HBM where a sequence has few rows: 64 sequences of 200 to 8192 keys, 32/8 heads
-// of 128, bf16: 118 us, 4.8 TB/s; two of 125000, fp16: 188 us, 5.7 TB/s; 48 of 1000 to
-// 32768 in MXFP4: 139 us, 4.3 TB/s beside the decoding. One of 500 keys is all latency,
+// of 128, bf16: 118 us, 4.9 TB/s; two of 125000, fp16: 190 us, 5.6 TB/s; 48 of 1000 to
+// 32768 in MXFP4: 140 us, 4.2 TB/s beside the decoding. One of 500 keys is all latency,
 // 10 us. fp32 products bound a few rows in fp32 (12 sequences of 5 tokens: 19.5 us).
 #pragma once
 
@@ -1148,9 +1148,10 @@ template <typename T> __global__ __launch_bounds__(kJoinThreads) void attn_paged
 // ---------------------------------------------------------------- host side
 
 // Rows of a block's tile, chosen by the rows a sequence has on average: 16 that the
-// waves split the keys of, or 128 that they share out. (fp32 q over more than 128 dims of
+// waves split the keys of, or 128 that they share out. fp32 q over more than 192 dims of
 // MXFP4 stays at 16: its three terms of q and P, 256 dims wide, do not fit the registers
-// of a wave with 32 rows.)
+// of a wave with 32 rows (3 x 300 tokens over 12000 keys, 16/4 heads: 802 us at 16 rows,
+// 903 at 128; at 192 dims 815 and 616).
 struct Plan {
   bool wide;
   int rows;           // of a tile
@@ -1166,8 +1167,8 @@ inline Plan plan_of(int64_t seqs, int64_t total, bool packed, int64_t kv_heads, 
                     int64_t capacity, bool f32, bool mxfp4) {
   Plan p{};
   const int64_t rows = total * group;
-  p.wide = packed && rows > 32 * seqs && !(f32 && mxfp4 && head_dim > 128);
-  p.rows = p.wide ? (f32 && head_dim > 128 ? 64 : 128) : 16;
+  p.wide = packed && rows > 32 * seqs && !(f32 && mxfp4 && head_dim > 192);
+  p.rows = p.wide ? (f32 && !mxfp4 && head_dim > 128 ? 64 : 128) : 16;
   p.tiles = packed ? rows / p.rows + seqs : seqs * ((group + p.rows - 1) / p.rows);
   if (p.tiles < 1) p.tiles = 1;
   p.min_chunk = 512;
