@@ -145,13 +145,17 @@ struct Item {
 };
 
 // Keys of a chunk, from the sum of row tiles times keys: an even share of the blocks that
-// run at once where that cuts the sequences into no more blocks than those, else a third of
-// it, so that blocks of different lengths fill each other's gaps. 48 sequences of 1000 to
-// 32768 keys in 4 bits, 8 heads: 159 us at an even share, 142 at half, 137 at a third, 153 at
-// a sixth; two of 131071 keys: 189, 198, 201 at the first three.
+// run at once where that cuts the sequences into no more blocks than those, or none of
+// them, else a third of it, so that blocks of different lengths fill each other's gaps. 48
+// sequences of 1000 to 32768 keys in 4 bits, 8 heads: 159 us at an even share, 142 at half,
+// 137 at a third, 153 at a sixth; two of 131071 keys: 189, 198, 201 at the first three. 128
+// of 1024 keys, which an even share leaves whole: 74.6 us cut, 45.4 whole (bf16 rows 118.9,
+// 104.8). A block of 4-bit keys starts in the time of many of them, so a third is at least
+// 2048 there: 48 of 4096 keys 58.8 -> 51.5. A sequence's chunks are as equal as steps allow:
+// 128 of 4096 keys 162 -> 135.
 constexpr int kParts = 3;
 
-template <int ROWS> __device__ __forceinline__ int chunk_of(const Args& a, float work) {
+template <int ROWS> __device__ __forceinline__ int chunk_of(const Args& a, float work, int tiles) {
   // 1.02: a fp32 sum of up to 2^18 terms a lane is off by less, and the room for partial sums counts on it
   const float even = fminf(work * 1.02f / a.target, 1e9f);
   const int keys = max(((int)even + 64) / 64 * 64, a.min_chunk);
@@ -163,7 +167,8 @@ template <int ROWS> __device__ __forceinline__ int chunk_of(const Args& a, float
   }
   blocks = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scan(blocks)), 63));
   return __builtin_amdgcn_readfirstlane(
-      blocks * a.kv_heads <= a.at_once ? keys : max(((int)(even / kParts) + 64) / 64 * 64, a.min_chunk));
+      blocks * a.kv_heads <= a.at_once || blocks == (float)tiles ? keys
+                                                                 : max(((int)(even / kParts) + 64) / 64 * 64, a.ks ? 2048 : 512));
 }
 
 // Which piece of work block x is, the same in every lane; seq < 0: none. Each wave
@@ -185,7 +190,7 @@ template <int ROWS> __device__ __forceinline__ Item find(const Args& a, int x) {
     }
     work = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scan(work)), 63));
     tiles = __builtin_amdgcn_readlane(scan(tiles), 63);
-    it.keys = chunk_of<ROWS>(a, work);
+    it.keys = chunk_of<ROWS>(a, work, tiles);
   }
   it.all_tiles = tiles;
   int before = 0, tiles_before = 0;
@@ -208,6 +213,11 @@ template <int ROWS> __device__ __forceinline__ Item find(const Args& a, int x) {
       it.s.n = __builtin_amdgcn_readlane(s.n, at);
       it.s.len = __builtin_amdgcn_readlane(s.len, at);
       it.splits = __builtin_amdgcn_readlane(splits, at);
+      if (it.splits > 1) {  // as equal as a block's steps allow
+        const unsigned unit = ROWS > 16 ? 32 : (a.ks ? 512 : 128);
+        const unsigned share = ((unsigned)it.s.len + (unsigned)it.splits - 1) / (unsigned)it.splits;
+        it.keys = min(it.keys, (int)((share + unit - 1) / unit * unit));
+      }
       const int k = rel - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(mine, at));
       const int tile = it.splits == 1 ? k : (int)((unsigned)k / (unsigned)it.splits);
       it.chunk = k - tile * it.splits;
@@ -336,6 +346,7 @@ template <typename T> __device__ __forceinline__ bool wild2(uint32_t w) {
 //   pv     O^T += V^T P^T of tiles 2 u and 2 u + 1  (32 keys)
 //   pv_apart  the same with every key's part added to the rows that see it alone
 //   wild   whether their values hold an Inf or a NaN
+// kTerms: P is the sum of two terms there and values may be an Inf.
 
 // Key 0 .. 31 of a product of 32 is row 4 (key / 16) + key % 4 of lane group (key % 16) / 4:
 // all ones there, in the lanes of that group, and zeros for the other rows.
@@ -364,7 +375,7 @@ __device__ __forceinline__ void add_if(bool in, const f32x4& x, f32x4& acc) {
 template <typename T_, int DL_> struct Rows16 {
   typedef T_ T;
   static constexpr int DL = DL_, VL = DL / 16, SUB = 1, QN = DL / 32, VH = VL > 8 ? 2 : 1;
-  static constexpr bool kMx = false;
+  static constexpr bool kMx = false, kTerms = true;
   struct Buf {
     w4 k[2][QN];
     uint32_t v[8][VL / 2];
@@ -448,7 +459,8 @@ template <typename T_, int DL_> struct Rows16 {
         for (int m = 0; m < 2; ++m) acc[r][e] = Mma16<T>::run(f, p[r][m], acc[r][e]);
     }
   }
-  // The same product one key at a time, added to the rows that see it: in(r, key).
+  // The same product one key at a time, added to the rows that see it: in(r, key). P's first
+  // term alone: an Inf times it and times a second one, 0 or of the other sign, is a NaN.
   template <int R, typename F>
   static __device__ __forceinline__ void pv_apart(const Buf& b, int, const Prob (&p)[R], f32x4 (&acc)[R][VL], const F& in) {
 #pragma unroll 1
@@ -461,20 +473,21 @@ template <typename T_, int DL_> struct Rows16 {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           f32x4 s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int m = 0; m < 2; ++m) s = Mma16<T>::run(f, only(p[r][m], mask), s);
+          s = Mma16<T>::run(f, only(p[r][0], mask), s);
           add_if(in(r, key), s, acc[r][e]);
         }
       }
     }
   }
   static __device__ __forceinline__ bool wild(const Buf& b, int) {
-    bool w = false;
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 top = {0, 0};
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int j = 0; j < VL / 2; ++j) w = w || wild2<T>(b.v[i][j]);
-    return w;
+      for (int w = 0; w < VL / 2; ++w) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, b.v[i][w] & 0x7fff7fffu));
+    constexpr unsigned short kInf = __is_same(T, bf16) ? 0x7f80 : 0x7c00;
+    return top.x >= kInf || top.y >= kInf;
   }
 };
 
@@ -491,7 +504,7 @@ template <int DL_> struct Rows32 {
   struct Prob {
     float p[8];
   };
-  static constexpr bool kMx = false;
+  static constexpr bool kMx = false, kTerms = false;
   const char *kb, *vb;
   int koff[QN], voff[4][VL / 4];
 
@@ -598,7 +611,7 @@ template <typename T_, int DL_> struct RowsMx {
   static constexpr int TERMS = sizeof(T) == 4 ? 3 : (__is_same(T, bf16) ? 1 : 2), PTERMS = sizeof(T) == 4 ? 3 : 2;
   static constexpr int DL = DL_, VL = DL / 16, QN = DL / 32;
   static constexpr int SUB = DL <= 128 && TERMS == 1 ? 4 : 2, NT = 2 * SUB;
-  static constexpr bool kMx = true;
+  static constexpr bool kMx = true, kTerms = false;
   static constexpr int KW = DL >= 128 ? 4 : 2;     // words of codes in a K piece
   static constexpr int KP = DL >= 128 ? DL / 128 : 1;  // K pieces of a row in a lane
   static constexpr int VW = VL >= 8 ? VL / 8 : 1;  // words of codes of a V row in a lane (half a word at DL 64)
@@ -966,7 +979,8 @@ attn_paged_kernel(Args a) {
       }
       // Where some rows see a key that others do not, an Inf or a NaN among the values must
       // stay out of the others (0 times it is a NaN): such steps are left for the loop below.
-      if (!whole && key0 + KEYS > low && __any(C::wild(b, u))) left = true;
+      // So are they where P has two terms (kTerms) and a value may be an Inf.
+      if ((C::kTerms || (!whole && key0 + KEYS > low)) && __any(C::wild(b, u))) left = true;
       else C::template pv<R>(b, u, p, acc);
     }
     if (more) cache.load_v(lk, (i + 1) % PER * TILES, b);
@@ -977,7 +991,7 @@ attn_paged_kernel(Args a) {
   if (left)
     for (int i = 0; i < own; ++i) {
       const int key0 = k0 + step_of(i) * KEYS;
-      if (key0 + KEYS <= low) continue;
+      if (!C::kTerms && key0 + KEYS <= low) continue;
       lk = look(i);
       cache.load_k(lk, 0, b);
       cache.load_v(lk, 0, b);
@@ -1147,11 +1161,18 @@ template <typename T> __global__ __launch_bounds__(kJoinThreads) void attn_paged
 
 // ---------------------------------------------------------------- host side
 
-// Rows of a block's tile, chosen by the rows a sequence has on average: 16 that the
-// waves split the keys of, or 128 that they share out. fp32 q over more than 192 dims of
-// MXFP4 stays at 16: its three terms of q and P, 256 dims wide, do not fit the registers
-// of a wave with 32 rows (3 x 300 tokens over 12000 keys, 16/4 heads: 802 us at 16 rows,
-// 903 at 128; at 192 dims 815 and 616).
+// Rows of a block's tile: 16 that the waves split the keys of, or 128 that they share out,
+// where a sequence has more than 32 rows on average and the work is enough for the fewer
+// blocks: row tiles of 16 times keys (as many as the table holds) past 768 a block that
+// runs at once over 16-bit rows, 2048 over 4 bits and in fp32. One sequence of 128 rows a
+// kv head, 8 of them, 128 dims, bf16: 9 us at 16 rows, 16 at 128 over 256 keys, 16 and 26
+// over 1024, 34 and 30 over 8192; eight of 1024 rows over 8192: 1173 and 333; into 4 bits
+// with fp16 q 27 and 40, and 695 and 496. Over 270 such calls the choice costs 1 to 4 % of
+// the better side, always 128 rows 21 to 91 %. fp32 q over MXFP4 has three terms of q and P,
+// which leave a wave no second one beside it: 16 rows are as fast or faster (eight of 1024
+// rows over 8192 keys, 128 dims: 800 us against 959; 256 dims, 3 x 300 tokens over 12000
+// keys, 16/4 heads: 802, 903) but for 129 to 192 dims, for which that kernel has only rows
+// of 256 (192 dims: 815, 616).
 struct Plan {
   bool wide;
   int rows;           // of a tile
@@ -1167,12 +1188,13 @@ inline Plan plan_of(int64_t seqs, int64_t total, bool packed, int64_t kv_heads, 
                     int64_t capacity, bool f32, bool mxfp4) {
   Plan p{};
   const int64_t rows = total * group;
-  p.wide = packed && rows > 32 * seqs && !(f32 && mxfp4 && head_dim > 192);
+  p.at_once = 2 * cu_count();  // eight waves a CU, what their registers allow
+  p.wide = packed && rows > 32 * seqs && (double)(rows * kv_heads / 16) * capacity > p.at_once * (f32 || mxfp4 ? 2048. : 768.) &&
+           !(f32 && mxfp4 && (head_dim <= 128 || head_dim > 192));
   p.rows = p.wide ? (f32 && !mxfp4 && head_dim > 128 ? 64 : 128) : 16;
   p.tiles = packed ? rows / p.rows + seqs : seqs * ((group + p.rows - 1) / p.rows);
   if (p.tiles < 1) p.tiles = 1;
   p.min_chunk = 512;
-  p.at_once = 2 * cu_count();  // eight waves a CU, what their registers allow
   p.target = (int)((p.at_once + kv_heads - 1) / kv_heads);
   p.split = capacity > p.min_chunk && (!p.wide || p.tiles * kv_heads < p.at_once);
   p.items = p.tiles;

@@ -14,12 +14,14 @@ template <typename T, int DL> int launch_wide_mx(const Args& a, const Plan& p, h
 
 template <typename T> int launch_mx(const Args& a, const Plan& p, hipStream_t s, const char* who) {
   if (p.wide) {
-    if constexpr (sizeof(T) == 2)  // fp32 is not wide there (plan_of)
-      if (a.d > 192) return launch_wide_mx<T, 256>(a, p, s, who);
-    return a.d <= 64    ? launch_wide_mx<T, 64>(a, p, s, who)
-           : a.d <= 96  ? launch_wide_mx<T, 96>(a, p, s, who)
-           : a.d <= 128 ? launch_wide_mx<T, 128>(a, p, s, who)
-                        : launch_wide_mx<T, 192>(a, p, s, who);
+    if constexpr (sizeof(T) == 4)
+      return launch_wide_mx<T, 192>(a, p, s, who);  // nowhere else (plan_of)
+    else
+      return a.d <= 64    ? launch_wide_mx<T, 64>(a, p, s, who)
+             : a.d <= 96  ? launch_wide_mx<T, 96>(a, p, s, who)
+             : a.d <= 128 ? launch_wide_mx<T, 128>(a, p, s, who)
+             : a.d <= 192 ? launch_wide_mx<T, 192>(a, p, s, who)
+                          : launch_wide_mx<T, 256>(a, p, s, who);
   }
   return a.d <= 64    ? launch<RowsMx<T, 64>, 1, true>(a, p, s, who)
          : a.d <= 128 ? launch<RowsMx<T, 128>, 1, true>(a, p, s, who)

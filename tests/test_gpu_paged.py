@@ -25,6 +25,26 @@ def _device():
         pytest.skip("no HIP device")
 
 
+@pytest.fixture(autouse=True, params=["", "long-table"])
+def _long_table(request, monkeypatch):
+    """Every packed call also with a table that has room for 2^21 keys, which selects the kernel of many rows where a
+    sequence has more than 32 (and lets any call split its keys): the entries behind the test's are outside the pool."""
+    if not request.param:
+        return
+
+    def longer(op, at):
+        def call(*args, **kwargs):
+            args = list(args)
+            if len(args) > at + 2 and args[at + 2] is not None and args[at].dim() == 2:
+                room = (1 << 21) // max(args[1].shape[2], 16) - args[at].shape[1]
+                args[at] = torch.nn.functional.pad(args[at], (0, max(room, 0)), value=-1)
+            return op(*args, **kwargs)
+        return call
+
+    monkeypatch.setattr(impls, "attn_paged", longer(impls.attn_paged, 3))
+    monkeypatch.setattr(impls, "attn_paged_mxfp4", longer(impls.attn_paged_mxfp4, 5))
+
+
 def _run(lens, news, hq, hkv, d, ps, dtype, mxfp4=False, causal=True, scale=None, seed=0, spare=3, width=None, packed=None,
          table=None):
     """One call against float64. news None: one token each, without offsets."""
@@ -103,6 +123,14 @@ def test_split_keys(news, mxfp4):
     """Long sequences beside short ones: chunks joined by the second kernel."""
     _run([5000, 90], news, 8, 2, 64, 32, BF, mxfp4)
     _run([3100, 2049], news, 4, 4, 128, 16, F32, mxfp4, scale=0.3)
+
+
+@pytest.mark.parametrize("mxfp4", [False, True], ids=["rows", "mxfp4"])
+@pytest.mark.parametrize("dtype", [BF, F16, F32], ids=str)
+def test_many_row_tiles(dtype, mxfp4):
+    """512 blocks of 128 rows and more: one round of them, whose keys stay whole."""
+    _run([150, 40], [130, 2], 512, 64, 32, 16, dtype, mxfp4)
+    _run([70, 33], [35, 33], 1024, 64, 96, 16, dtype, mxfp4)
 
 
 def test_many_sequences():
@@ -202,6 +230,24 @@ def test_nonfinite_keys_reach_only_the_tokens_that_see_them(dtype, where):
     else:
         assert (got[blind:, 2:, 5] == INF).all() and got[blind:, 2:, :5].isfinite().all()
         assert got4[blind:, 2:, :32].isnan().all() and got4[blind:, 2:, 32:].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32], ids=str)
+@pytest.mark.parametrize("news", [[1, 1], [20, 3], [300, 3]], ids=str)
+def test_infinite_values_are_infinite_results(dtype, news):
+    """An Inf among the values of a key that every token sees: P times it is that Inf, in whatever terms P is held."""
+    ps, d, lens = 16, 64, [400, 30]
+    k, v = cache_of(27, 2, ps, d, dtype, 4)
+    table = table_of(lens, ps, 27, 25, 5)
+    total = sum(news)
+    q = torch.randn(total, 4, d, generator=torch.Generator().manual_seed(3)).to(dtype).mul_(0.25).to(DEV)
+    cu = torch.tensor([0, news[0], total], dtype=torch.int32)
+    v[table[0, 2], 1, 5, 7], v[table[1, 0], 0, 3, 9] = INF, -INF
+    got = impls.attn_paged(q, k.to(DEV), v.to(DEV), table.to(DEV), torch.tensor(lens, dtype=torch.int32).to(DEV), cu.to(DEV)).cpu()
+    first, second = got[:news[0]], got[news[0]:]
+    assert (first[:, 2:, 7] == INF).all() and (second[:, :2, 9] == -INF).all()
+    first[:, 2:, 7], second[:, :2, 9] = 0, 0
+    assert got.isfinite().all()
 
 
 def test_rows_without_a_finite_score():

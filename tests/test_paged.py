@@ -401,7 +401,8 @@ def test_workspace_queries(lib):
             assert ask(4, 4, 0, 32, 8, 128, 512, dtype, mxfp4) == 0  # one chunk at most
             assert ask(4, 4, 0, 32, 8, 128, 4096, dtype, mxfp4) > 0
             # a grid that fills the device without splitting: 262144 rows x 8 heads in tiles of 128
-            assert ask(4, 65536, 1, 32, 8, 128, 131072, dtype, mxfp4) == 0
+            if not (mxfp4 and dtype == _lib.F32):  # 16 rows a tile
+                assert ask(4, 65536, 1, 32, 8, 128, 131072, dtype, mxfp4) == 0
             for bad in ((-1, 4, 0, 32, 8, 128, 64), (4, 4, 0, 30, 8, 128, 64), (4, 4, 0, 32, 0, 128, 64),
                         (4, 1 << 30, 1, 32, 8, 128, 64), (4, 4, 0, 32, 8, 128, -1)):
                 assert ask(*bad, dtype, mxfp4) == -1, bad
