@@ -33,9 +33,9 @@
 // other lengths.
 //
 // Bound by HBM where a sequence has few rows: 64 sequences of 200 to 8192 keys, 32/8 heads
-// of 128, bf16: 118 us, 4.9 TB/s; two of 125000, fp16: 190 us, 5.6 TB/s; 48 of 1000 to
-// 32768 in MXFP4: 140 us, 4.2 TB/s beside the decoding. One of 500 keys is all latency,
-// 10 us. fp32 products bound a few rows in fp32 (12 sequences of 5 tokens: 19.5 us).
+// of 128, bf16: 118 us, 4.8 TB/s; two of 125000, fp16: 188 us, 5.7 TB/s; 48 of 1000 to
+// 32768 in MXFP4: 141 us, 4.2 TB/s beside the decoding. One of 500 keys is all latency,
+// 9 us. fp32 products bound a few rows in fp32 (12 sequences of 5 tokens: 20 us).
 #pragma once
 
 #include <math.h>

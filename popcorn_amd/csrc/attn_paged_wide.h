@@ -22,9 +22,9 @@
 // q and P enter as TERMS values of E (attn_paged.h): one where E is q's own type.
 //
 // 4 x 8192 tokens of 32/8 heads of 128, causal, bf16: 2227 us, 988 TFLOP/s. Chunks of 2048
-// tokens over 4096 to 8192 keys, four of them: 406 us, 835 TFLOP/s, the rest being the last
-// of 880 blocks. 300 fp16 tokens over 20011 keys in MXFP4, 28/4 heads of 96: 233 us
-// (253 in rows of 128).
+// tokens over 4096 to 8192 keys, four of them: 412 us, 821 TFLOP/s, the rest being the last
+// of 880 blocks. 300 fp16 tokens over 20011 keys in MXFP4, 28/4 heads of 96: 226 us
+// (20 more in rows of 128).
 #pragma once
 
 #include "attn_paged.h"
