@@ -19,7 +19,10 @@
 // one sequence of products whose LDS fragments are read kRing products ahead; K(t + 2) and
 // V(t + 1) are asked for at its start and there at its end, at one barrier a step.
 //
-// q and P enter as TERMS values of E (attn_paged.h): one where E is q's own type.
+// q and P enter as TERMS values of E (attn_paged.h): one where E is q's own type, as in the
+// forward of whole sequences. P is then rounded once, by half a step of E at most, which
+// many rows can bear beside the output's own rounding (bf16: 0.0023 of the values' size
+// against 0.0017 from the output alone); a second term would be half as many products again.
 //
 // 4 x 8192 tokens of 32/8 heads of 128, causal, bf16: 2227 us, 988 TFLOP/s. Chunks of 2048
 // tokens over 4096 to 8192 keys, four of them: 412 us, 821 TFLOP/s, the rest being the last
